@@ -484,6 +484,64 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
                               int *num_voxels_dev, int *overflow_dev, void *ws, size_t ws_bytes,
                               void *stream);
 
+/* ------------------------------------------------------------------ token operators -- */
+
+/* Layers over rows of features (BEV cells, object queries): what the transformer blocks that consume
+ * the LiDAR map are made of.  Storage is fp32, fp16 or bf16; all sums are fp32 and a value is rounded
+ * once, when it is stored.  Nothing here uses atomics: the same inputs give the same bits.  Rows are
+ * contiguous unless a row distance is an argument; no pointer needs more than its element's alignment
+ * (16-byte aligned rows of a multiple of 16 bytes are faster).  Outputs must not overlap inputs. */
+#define SF_DTYPE_F32 0
+#define SF_DTYPE_F16 1
+#define SF_DTYPE_BF16 2
+
+#define SF_ACT_NONE 0
+#define SF_ACT_RELU 1
+#define SF_ACT_GELU 2 /* z/2 (1 + erf(z / sqrt(2))) */
+
+/* Bytes of scratch sf_linear needs (0 for most sizes). */
+SF_API size_t sf_linear_workspace(long long m, long long k, long long n, int dtype);
+
+/* y = act(x weight^T + bias) + residual, one launch (two when few rows meet a long k).
+ *   x (m, k), rows ldx >= k elements apart;  weight (n, k);  bias (n) or NULL;
+ *   residual (m, n) or NULL;  y (m, n);  pre (m, n) or NULL: the values before the activation, which
+ *   sf_linear_backward takes.  All of one dtype.  m, k, n may be 0. */
+SF_API int sf_linear(const void *x, long long ldx, const void *weight, const void *bias,
+                     const void *residual, void *y, void *pre, long long m, long long k, long long n,
+                     int dtype, int act, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of scratch sf_linear_backward needs. */
+SF_API size_t sf_linear_backward_workspace(long long m, long long k, long long n, int dtype, int act);
+
+/* Gradients of sf_linear for the gradient dy (m, n) of y:
+ *   dz = dy act'(pre);  dx (m, k) = dz weight;  dw (n, k) = dz^T x;  db (n) = sum of dz's rows.
+ * dx, dw and db may each be NULL (not wanted).  pre is not read when act is SF_ACT_NONE.  The
+ * residual's gradient is dy itself.  dz is held in dtype between the passes (the products take it as
+ * an operand); db sums it unrounded. */
+SF_API int sf_linear_backward(const void *dy, const void *x, long long ldx, const void *weight,
+                              const void *pre, void *dx, void *dw, void *db, long long m, long long k,
+                              long long n, int dtype, int act, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* s = x + residual;  y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over rows of d elements
+ * (var: the mean square, no Bessel correction).
+ *   x, residual (or NULL), y, sum (s rounded, or NULL): (m, d) of dtype;  weight, bias (d) or NULL:
+ *   of param_dtype, dtype or fp32;  mean, rstd (m) fp32 or NULL: what the backward pass takes. */
+SF_API int sf_layer_norm(const void *x, const void *residual, const void *weight, const void *bias,
+                         void *y, void *sum, float *mean, float *rstd, long long m, int d, float eps,
+                         int dtype, int param_dtype, void *stream);
+
+/* Bytes of scratch sf_layer_norm_backward needs for dw / db. */
+SF_API size_t sf_layer_norm_backward_workspace(long long m, int d, int dtype);
+
+/* Gradients of sf_layer_norm: x is the normalised sum s, dy the gradient of y, dsum (or NULL) the
+ * gradient that reaches s directly.  dx (m, d) is the gradient of s, hence of x and of residual;
+ * dw, db (d) of param_dtype, each NULL when not wanted. */
+SF_API int sf_layer_norm_backward(const void *dy, const void *x, const float *mean, const float *rstd,
+                                  const void *weight, const void *dsum, void *dx, void *dw, void *db,
+                                  long long m, int d, int dtype, int param_dtype, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -99,6 +99,15 @@ SIGNATURES = {
     'sf_dynamic_scatter_workspace': (_sz, [C.POINTER(C.c_int), _i]),
     'sf_dynamic_scatter': (_i, [_vp, _vp, _i, _i, _i, C.POINTER(C.c_int), _i, _vp, _vp, _vp, _vp,
                                 _i, _vp, _vp, _vp, _sz, _vp]),
+    'sf_linear_workspace': (_sz, [_ll, _ll, _ll, _i]),
+    'sf_linear': (_i, [_vp, _ll, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp, _sz, _vp]),
+    'sf_linear_backward_workspace': (_sz, [_ll, _ll, _ll, _i, _i]),
+    'sf_linear_backward': (_i, [_vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp,
+                                _sz, _vp]),
+    'sf_layer_norm': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, C.c_float, _i, _i, _vp]),
+    'sf_layer_norm_backward_workspace': (_sz, [_ll, _i, _i]),
+    'sf_layer_norm_backward': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _ll, _i, _i, _i, _vp,
+                                    _sz, _vp]),
 }
 
 
@@ -167,6 +176,67 @@ def require(t, dtype, what):
     if t.dtype != dtype:
         raise RuntimeError(f'{what} must be {dtype}, got {t.dtype}')
     return t
+
+
+# storage types of the token operators (include/sparsefusion_hip.h: SF_DTYPE_*)
+DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class _Here:
+    """Context of a call whose device is the current one already."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        pass
+
+
+_HERE_ALREADY = _Here()
+
+
+def on(device):
+    """Context in which `device` is the current one: kernels launch, and outputs and scratch are
+    allocated, on the tensors' own device."""
+    if device.type != 'cuda':
+        raise RuntimeError('sparsefusion_amd ops need tensors on a HIP device '
+                           f'(got {device}); there is no CPU path')
+    if device.index == torch.cuda.current_device():
+        return _HERE_ALREADY
+    return torch.cuda.device(device)
+
+
+def same(x, **others):
+    """Refuse tensors of another type or on another device than x."""
+    for name, t in others.items():
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise RuntimeError(f'{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}')
+
+
+def rows(x):
+    """(..., K) as (M, K) with adjacent elements and evenly spaced rows, and their distance; a copy
+    only where the strides do not allow a view."""
+    k = x.shape[-1]
+    flat = x.reshape(x.numel() // k if k else x.shape[:-1].numel(), k)
+    if k > 1 and flat.stride(1) != 1 or flat.shape[0] > 1 and flat.stride(0) < k:
+        flat = flat.contiguous()
+    return flat, flat.stride(0) if flat.shape[0] > 1 else k
+
+
+def dev_ptr(t):
+    """ptr() for a tensor whose row distance is handed over with it."""
+    if not t.is_cuda:
+        return ptr(t)
+    return t.data_ptr()
+
+
+def workspace(nbytes, device):
+    """(tensor, size) of scratch memory from the caching allocator, (None, 0) for none.  The block
+    returns to the current stream's pool when the caller drops it and is handed out again in that
+    stream's order only; under capture it belongs to the graph's own pool."""
+    if not nbytes:
+        return None, 0
+    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
 
 
 class _ForwardOnly(torch.autograd.Function):

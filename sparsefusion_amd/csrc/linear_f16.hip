@@ -1,0 +1,7 @@
+// The matrix products of the linear layer for f16 operands (gemm_tile.h); a file of its own per
+// storage type so that the kernels compile side by side.
+#include "gemm_tile.h"
+
+void sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st) {
+  sf_gemm_any<_Float16>(a, layout, tile, dma, st);
+}

@@ -55,6 +55,11 @@ static __global__ void sf_fill_u32_kernel(uint32_t *__restrict__ p, size_t n, ui
        i += (size_t)gridDim.x * blockDim.x)
     p[i] = v;
 }
+static __global__ void sf_fill_u16_kernel(uint16_t *__restrict__ p, size_t n, uint16_t v) {
+  for (size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (size_t)gridDim.x * blockDim.x)
+    p[i] = v;
+}
 #define SF_FILL_U32(ptr, n_words, value, st)                                                      \
   do {                                                                                            \
     if ((size_t)(n_words) > 0) {                                                                  \

@@ -1,0 +1,162 @@
+"""Layer norm over the last dimension, with the residual add in front of it, and its gradients.
+
+`LayerNorm` is `nn.LayerNorm` over one dimension (same arguments, parameters and state-dict keys)
+whose forward runs `sf_layer_norm` (csrc/layer_norm.hip); it is registered as the norm layer `LN`, so
+`norm_cfg=dict(type='LN')` reaches it in every module that builds its norms from a config (sparse conv
+blocks apply it to the (N, C) voxel features).  Rows are fp32, fp16 or bf16, parameters of the same
+type or fp32; statistics and sums are fp32 and every output is rounded once.  Differentiable once (no
+double backward).  No CPU path.
+"""
+import torch
+from torch import nn
+
+from . import _lib
+from .registry import NORM_LAYERS
+
+
+def _check(x, weight, bias):
+    if x.dtype not in _lib.DTYPE_CODES:
+        raise RuntimeError(f'layer_norm takes fp32, fp16 or bf16, got {x.dtype}')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f'layer_norm needs rows of at least one element, got {tuple(x.shape)}')
+    d = x.shape[-1]
+    dtype = None
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (d,):
+            raise RuntimeError(f'{name} must have shape ({d},), got {tuple(t.shape)}')
+        if t.device != x.device:
+            raise RuntimeError(f'{name} is on {t.device}, x on {x.device}')
+        if t.dtype not in (x.dtype, torch.float32) or t.dtype != (dtype or t.dtype):
+            raise RuntimeError(f'weight and bias must both be {x.dtype} or both float32, '
+                               f'{name} is {t.dtype}')
+        dtype = t.dtype
+    return dtype or x.dtype
+
+
+def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=False,
+                       keep_stats=False):
+    """-> (y, sum, mean, rstd) of s = x + residual, y = (s - mean) * rstd * weight + bias.  sum (s
+    rounded) with return_sum, mean and rstd (fp32, x.shape[:-1]) with keep_stats, else None.  Not
+    differentiable: see `layer_norm`."""
+    pdtype = _check(x, weight, bias)
+    if not eps >= 0:
+        raise RuntimeError(f'eps must not be negative, got {eps}')
+    d = x.shape[-1]
+    if residual is not None:
+        _lib.same(x, residual=residual)
+        if residual.shape != x.shape:
+            residual = residual.expand(x.shape)
+        residual = residual.contiguous()
+    x = x.contiguous()
+    m = x.numel() // d
+    with _lib.on(x.device):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_sum else None
+        mean = rstd = None
+        if keep_stats:
+            mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        _lib.check(_lib.lib().sf_layer_norm(
+            _lib.ptr(x), _lib.ptr(residual), _lib.ptr(weight.contiguous()) if weight is not None else None,
+            _lib.ptr(bias.contiguous()) if bias is not None else None, y.data_ptr(), _lib.ptr(s),
+            _lib.ptr(mean), _lib.ptr(rstd), m, d, eps, _lib.DTYPE_CODES[x.dtype],
+            _lib.DTYPE_CODES[pdtype], _lib.stream(x.device)))
+    return y, s, mean, rstd
+
+
+def layer_norm_backward(grad, x, mean, rstd, weight=None, grad_sum=None, needs=(True, True, True),
+                        param_dtype=None):
+    """Gradients (dx, dweight, dbias) of `layer_norm_forward` for the gradient `grad` of y and
+    `grad_sum` of the sum (or None); x is the normalised sum, mean and rstd as it returned them.  dx is
+    the gradient of x and of the residual alike.  `needs` says which are wanted, the others are None;
+    the parameter gradients have weight's type (without a weight: `param_dtype`, or x's)."""
+    pdtype = _check(x, weight, None)
+    if weight is None and param_dtype is not None:
+        pdtype = param_dtype
+        if pdtype not in (x.dtype, torch.float32):
+            raise RuntimeError(f'param_dtype must be {x.dtype} or float32, got {pdtype}')
+    _lib.same(x, grad=grad, grad_sum=grad_sum)
+    d = x.shape[-1]
+    for name, t in (('grad', grad), ('grad_sum', grad_sum)):
+        if t is not None and t.shape != x.shape:
+            raise RuntimeError(f'{name} must have shape {tuple(x.shape)}, got {tuple(t.shape)}')
+    m = x.numel() // d
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        if t.dtype != torch.float32 or t.numel() != m or t.device != x.device:
+            raise RuntimeError(f'{name} must be {m} fp32 values on {x.device}, got {tuple(t.shape)} '
+                               f'{t.dtype} on {t.device}')
+    grad, x = grad.contiguous(), x.contiguous()
+    grad_sum = grad_sum.contiguous() if grad_sum is not None else None
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    with _lib.on(x.device):
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dw = torch.empty((d,), dtype=pdtype, device=x.device) if needs[1] else None
+        db = torch.empty((d,), dtype=pdtype, device=x.device) if needs[2] else None
+        dtype = _lib.DTYPE_CODES[x.dtype]
+        L = _lib.lib()
+        need = L.sf_layer_norm_backward_workspace(m, d, dtype) if needs[1] or needs[2] else 0
+        ws, nbytes = _lib.workspace(need, x.device)
+        _lib.check(L.sf_layer_norm_backward(
+            _lib.ptr(grad), _lib.ptr(x), _lib.ptr(mean), _lib.ptr(rstd),
+            _lib.ptr(weight.contiguous()) if weight is not None else None, _lib.ptr(grad_sum),
+            dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), m, d, dtype, _lib.DTYPE_CODES[pdtype],
+            _lib.ptr(ws), nbytes, _lib.stream(x.device)))
+    return dx if needs[0] else None, dw, db
+
+
+class _LayerNorm(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, residual, return_sum):
+        y, s, mean, rstd = layer_norm_forward(x, weight, bias, eps, residual,
+                                              return_sum or residual is not None, True)
+        ctx.pdtype = bias.dtype if bias is not None else None
+        ctx.set_materialize_grads(False)
+        # without a residual the sum is x: a returned one is x's copy, the saved one x itself
+        ctx.save_for_backward(x if residual is None else s, weight, mean, rstd)
+        return (y, s) if return_sum else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, grad_sum=None):
+        x, weight, mean, rstd = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        if grad is None and grad_sum is None:
+            return (None,) * 6
+        if grad is None:
+            grad = torch.zeros_like(x)
+        dx, dw, db = layer_norm_backward(grad, x, mean, rstd, weight, grad_sum,
+                                         (needs[0] or needs[4], needs[1], needs[2]), ctx.pdtype)
+        return dx if needs[0] else None, dw, db, None, dx if needs[4] else None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=False):
+    """Layer norm of x + residual over the last dimension, differentiable in all four tensors; with
+    return_sum -> (y, sum), for blocks that carry the sum on.  weight and bias (D,) or None; residual
+    has x's shape or expands to it (its gradient is summed back)."""
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        if residual is not None and residual.shape != x.shape:
+            residual = residual.expand(x.shape)
+        return _LayerNorm.apply(x, weight, bias, eps, residual, return_sum)
+    y, s, _, _ = layer_norm_forward(x, weight, bias, eps, residual, return_sum)
+    return (y, s) if return_sum else y
+
+
+@NORM_LAYERS.register_module('LN')
+class LayerNorm(nn.LayerNorm):
+    """`nn.LayerNorm` over the last dimension with an optional residual added in front."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, device=None,
+                 dtype=None):
+        super().__init__(normalized_shape, eps, elementwise_affine, bias, device=device, dtype=dtype)
+        if len(self.normalized_shape) != 1:
+            raise NotImplementedError('LayerNorm over more than the last dimension')
+
+    def forward(self, x, residual=None, return_sum=False):
+        if tuple(x.shape[-1:]) != self.normalized_shape:
+            raise RuntimeError(f'expected rows of {self.normalized_shape[0]} elements, got '
+                               f'{tuple(x.shape)}')
+        return layer_norm(x, self.weight, self.bias, self.eps, residual, return_sum)

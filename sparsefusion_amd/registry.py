@@ -41,6 +41,7 @@ CONV_LAYERS = Registry('conv layer')
 NORM_LAYERS = Registry('norm layer')
 MIDDLE_ENCODERS = Registry('middle_encoder')
 VOXEL_ENCODERS = Registry('voxel_encoder')
+LINEAR_LAYERS = Registry('linear layer')
 
 NORM_LAYERS.register_module('BN1d', module=nn.BatchNorm1d)
 NORM_LAYERS.register_module('BN', module=nn.BatchNorm2d)
@@ -57,7 +58,8 @@ def build_conv_layer(cfg, *args, **kwargs):
 
 
 def build_norm_layer(cfg, num_features, postfix=''):
-    """mmcv.cnn.build_norm_layer -> (name, layer); abbreviation 'bn' as mmcv infers for BN*."""
+    """mmcv.cnn.build_norm_layer -> (name, layer); abbreviations 'bn' and 'ln' as mmcv infers them."""
+    from . import layer_norm  # noqa: F401  (registers LN)
     cfg = dict(cfg)
     cls = NORM_LAYERS.get(cfg.pop('type'))
     if cls is None:
@@ -67,7 +69,17 @@ def build_norm_layer(cfg, num_features, postfix=''):
     layer = cls(num_features, **cfg)
     for p in layer.parameters():
         p.requires_grad = requires_grad
-    return 'bn' + str(postfix), layer
+    return ('ln' if isinstance(layer, nn.LayerNorm) else 'bn') + str(postfix), layer
+
+
+def build_linear_layer(cfg, *args, **kwargs):
+    """mmcv.cnn.build_linear_layer: cfg = dict(type='Linear', activation='relu')."""
+    from . import linear  # noqa: F401  (registers Linear)
+    cfg = dict(cfg)
+    cls = LINEAR_LAYERS.get(cfg.pop('type'))
+    if cls is None:
+        raise KeyError('unknown linear layer type')
+    return cls(*args, **kwargs, **cfg)
 
 
 def _populate():
