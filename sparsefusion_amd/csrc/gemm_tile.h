@@ -12,9 +12,10 @@
 //
 // A workgroup owns a BP x BQ tile and walks k in steps of 128 bytes (64 16-bit or 32 fp32 elements).
 // Both operands' tiles go to LDS in 16-byte chunks, straight from memory (buffer_load ... lds) when
-// every chunk is aligned and whole, through registers otherwise; two buffers, the next step's loads
-// in flight while this one multiplies.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32;
-// Q is the instruction's first operand, so a lane ends up with four consecutive q of one row p.
+// every chunk is aligned and whole, through registers otherwise; two buffers, the loads two steps
+// ahead.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32; Q is the instruction's first
+// operand, so a lane ends up with four consecutive q of one row p.  Workgroups stay and walk the
+// tiles: the loads of the next tile's first steps run under the epilogue of the last.
 // Rows and k outside the operands read as zeros (the buffer descriptor's range check), columns
 // outside are never stored.
 //
@@ -31,16 +32,48 @@ typedef short sf_s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
+// Phi(z), the normal distribution function, as 1 / (1 + exp(-z P(z^2))): P fits logit(Phi(z)) / z
+// over |z| <= 6, its coefficients (by powers of z^2) for the least maximal error of Phi; the leading
+// one is positive, so farther out Phi runs into 0 or 1.  fp32: seven coefficients, 2.9e-8 off (half a
+// step of fp32 at 1 is 6e-8); 16-bit outputs: five, 1.4e-6 off (half a step of fp16 at 1 is 2.4e-4).
+// 18 and 16 instruction slots (exp and rcp take four each) against about 45 of
+// 0.5 (1 + erff(z / sqrt(2))), whose two branches both run in most waves: the layer of
+// 32400 x 256 -> 1024 went from 68 to 47 us with it.  With the fp32 evaluation 1.3e-7 and 1.6e-6 off.
+// The coefficients carry -log2(e) for v_exp_f32.
+template <typename T>
+__device__ __forceinline__ float sf_phi(float z) {
+  constexpr float kL = -1.4426950408889634f;
+  const float q = z * z;
+  float p;
+  if constexpr (sizeof(T) == 4) {
+    p = 3.51255832e-09f * kL;
+    p = fmaf(p, q, -2.64532672e-07f * kL);
+    p = fmaf(p, q, 7.92954762e-06f * kL);
+    p = fmaf(p, q, -1.10612640e-04f * kL);
+    p = fmaf(p, q, -6.51894754e-05f * kL);
+    p = fmaf(p, q, 7.26661688e-02f * kL);
+    p = fmaf(p, q, 1.59576988e+00f * kL);
+  } else {
+    p = 2.85001296e-06f * kL;
+    p = fmaf(p, q, -7.33869147e-05f * kL);
+    p = fmaf(p, q, -1.75652994e-04f * kL);
+    p = fmaf(p, q, 7.27845723e-02f * kL);
+    p = fmaf(p, q, 1.59573942e+00f * kL);
+  }
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p * z));
+}
+template <typename T>
 __device__ __forceinline__ float sf_act(float z, int act) {
   if (act == SF_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (act == SF_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (act == SF_ACT_GELU) return z * sf_phi<T>(z);
   return z;
 }
+template <typename T>
 __device__ __forceinline__ float sf_act_slope(float z, int act) {
   if (act == SF_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == SF_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-           z * (__expf(-0.5f * z * z) * 0.39894228040143268f);
+  if (act == SF_ACT_GELU)      // Phi(z) + z phi(z)
+    return fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f),
+                sf_phi<T>(z));
   return 1.0f;
 }
 
@@ -78,104 +111,140 @@ template <> struct SfMfma<__bf16> {
   }
 };
 
-// One operand's side of the tile: B rows of the output, KMINOR as above.
-template <typename T, bool KMINOR, int B, int WAVES, bool DMA>
+// 16 bytes per lane straight into LDS, lane L's to lds + 16 L (wave-uniform), zeros for an offset out
+// of rs's range.  Written as assembly because the compiler makes every LDS read that it cannot tell
+// from the destination wait for the builtin form, all of it, and these loads are meant to stay in
+// flight under such reads.  Nothing comes back in registers; who reads the destination waits for
+// vmcnt(0) by hand and meets the other waves at a barrier.  (The compiler's own counted waits only
+// become stricter: vmcnt retires in order.)
+// `lds` + OFFSET goes to m0; the wait states cover an SGPR that a vector instruction wrote just before.
+template <int OFFSET>
+__device__ __forceinline__ void sf_lds_load16(const sf_u32x4 &rs, unsigned lds, unsigned off) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"((unsigned)__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(rs), "i"(OFFSET)
+               : "m0", "scc", "memory");
+#endif
+}
+
+// One operand's side of the tile: B rows of the output, KMINOR as above, STEP bytes of a row's k (128
+// or 64) brought at a time.
+template <typename T, bool KMINOR, int B, int WAVES, int STEP, bool DMA>
 struct SfOperand {
-  static constexpr int S = sizeof(T), V = 16 / S, BK = 128 / S;
-  static constexpr int CPR = KMINOR ? B * S / 16 : 8;     // chunks of one LDS row
+  static constexpr int S = sizeof(T), V = 16 / S, BK = STEP / S;
+  static constexpr int CPR = KMINOR ? B * S / 16 : STEP / 16;     // chunks of one LDS row
   static constexpr int ROWB = CPR * 16;
   static constexpr int RPI = 64 / CPR;                    // LDS rows one wave-instruction fills
-  static constexpr int NI = B * 128 / 1024 / WAVES;       // instructions of a wave a k step
-  static_assert(CPR <= 64 && NI >= 1 && NI * WAVES * 1024 == B * 128, "tile shape");
+  static constexpr int NI = B * STEP / 1024 / WAVES;      // instructions of a wave a step
+  static_assert(CPR <= 64 && NI >= 1 && NI * WAVES * 1024 == B * STEP, "tile shape");
   typedef typename SfMfma<T>::frag frag;
 
   static __device__ __forceinline__ int swz(int row) {
-    if constexpr (!KMINOR) return (row ^ (row >> 3)) & 7;
+    if constexpr (!KMINOR && STEP == 128) return (row ^ (row >> 3)) & 7;
+    else if constexpr (!KMINOR) return (row >> 3) & 3;
     else if constexpr (S == 4) return ((row >> 2) & 1) << 3;
     else if constexpr (CPR == 8) return ((row >> 1) & 1) << 2;
     else return (row & 3) << 2;
   }
 
-  const T *base;            // start of this workgroup's rows / columns, at k = 0
-  long long ld, nk;
-  long long rows;           // output rows this operand has from `base` on
-  unsigned voff[NI];        // byte offset of this lane's chunk from the step's start
-  short along[NI];          // K-major: the chunk's k; K-minor: its first output row
+  const T *at;              // the step being loaded: the tile's first row / column at its k
+  long long rows;           // output rows this operand has from the tile's first on
+  long long ld;
+  int steps, last_k;        // steps to go in this tile, k of its last one
+  unsigned range, range_last;       // DMA: bytes from `at` to the last element of a step in use
+  unsigned voff[DMA ? NI : 1];      // DMA: byte offset of this lane's chunk from `at`
+  int along[NI];            // K-major: the chunk's k; K-minor: its first output row
   sf_u32x4 reg[DMA ? 1 : NI];
 
-  __device__ __forceinline__ void init(const void *ptr, long long ld_, long long first,
-                                       long long total, long long nk_, int wave, int lane) {
-    ld = ld_, nk = nk_, rows = total - first;
-    base = static_cast<const T *>(ptr) + (KMINOR ? first : first * ld_);
+  __device__ __forceinline__ void init(long long ld_, int wave, int lane) {
+    ld = ld_;
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
       const int row = (j * WAVES + wave) * RPI + lane / CPR;
       const int c = (lane % CPR) ^ swz(row);
-      along[j] = (short)(c * V);
-      voff[j] = DMA ? (unsigned)((long long)row * ld * S) + c * 16u : (unsigned)row;
+      along[j] = c * V;
+      if constexpr (DMA) voff[j] = (unsigned)((long long)row * ld * S) + c * 16u;
     }
   }
-
-  // Bring the step at k0 towards `lds`: the whole way when DMA, into registers otherwise.
-  __device__ __forceinline__ void load(long long k0, unsigned char *lds, int wave) {
-    const long long left_k = nk - k0;
+  // A tile: output rows `first` on (of `total`), k from k0 on in `steps` steps, the last of last_k.
+  __device__ __forceinline__ void open(const void *ptr, long long first, long long total, long long k0,
+                                       int steps_, int last_k_) {
+    rows = total - first;
+    steps = steps_, last_k = last_k_;
+    at = static_cast<const T *>(ptr) + (KMINOR ? first + k0 * ld : first * ld + k0);
     if constexpr (DMA) {
-#if defined(__HIP_DEVICE_COMPILE__)
-      // the range ends with the last element in use, so every row past it reads as zeros; a chunk
-      // past the contiguous extent is sent out of range by hand (0x80000000 exceeds any range here)
-      const T *at = base + (KMINOR ? k0 * ld : k0);
-      long long n = KMINOR ? (left_k < BK ? left_k : BK) : (rows < B ? rows : B);
-      const long long last = KMINOR ? rows : left_k;
-      const long long bytes = ((n - 1) * ld + last) * S;
-      const unsigned range = bytes < 0x7FFFFFFF ? (unsigned)bytes : 0x7FFFFFFFu;
-      const __amdgpu_buffer_rsrc_t rs =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(at), 0, range, 0x00020000);
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const unsigned off = along[j] < last ? voff[j] : 0x80000000u;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (__attribute__((address_space(3))) void *)(lds + (j * WAVES + wave) * 1024), 16, off,
-            0, 0, 0);
-      }
-#endif
-    } else {
-#pragma unroll
-      for (int j = 0; j < NI; ++j) {
-        const int row = (int)voff[j], c = along[j];
-        const long long n = KMINOR ? left_k : rows;                     // rows there are
-        const long long m = (KMINOR ? rows : left_k) - c;               // elements from the chunk on
-        const T *at = base + (KMINOR ? (k0 + row) * ld : row * ld + k0) + c;
-        sf_u32x4 v = {0, 0, 0, 0};
-        if (row < n && m > 0) {
-          if (m >= V) {
-            v = *reinterpret_cast<const sf_u32x4_any *>(at);
-          } else {
-            typename SfMfma<T>::frag e;
-#pragma unroll
-            for (int i = 0; i < V; ++i) e[i] = i < m ? at[i] : (T)0.0f;
-            v = __builtin_bit_cast(sf_u32x4, e);
-          }
-        }
-        reg[j] = v;
+      // rows past the range read as zeros (the host sees to it that all of this fits 31 bits)
+      const int n = rows < B ? (int)rows : B;
+      if constexpr (KMINOR) {
+        range = (unsigned)(((BK - 1) * ld + rows) * S);
+        range_last = (unsigned)(((last_k - 1) * ld + rows) * S);
+      } else {
+        range = (unsigned)(((n - 1) * ld + BK) * S);
+        range_last = (unsigned)(((n - 1) * ld + last_k) * S);
       }
     }
   }
-  // Registers to LDS (nothing to do when the load went there itself).
-  __device__ __forceinline__ void store(unsigned char *lds, int wave, int lane) {
-    if constexpr (!DMA) {
-#pragma unroll
-      for (int j = 0; j < NI; ++j)
-        *reinterpret_cast<sf_u32x4 *>(lds + (j * WAVES + wave) * 1024 + lane * 16) = reg[j];
-    }
+  __device__ __forceinline__ void close() {      // nothing left to load: zeros from here on
+    range = range_last = 0;
+    steps = 0x7FFFFFFF;
   }
 
-  // Fragment of the 32 output rows at row0 for quarter s of the step: this lane's row is
+  // DMA of instruction J of the step towards LDS address `lds`; next() goes on to the following step.
+  // A chunk past the contiguous extent is sent out of range by hand (the others are past a row's end).
+  template <int J>
+  __device__ __forceinline__ void issue(unsigned lds_wave) const {
+    const unsigned long long addr = (unsigned long long)at;
+    const sf_u32x4 rs = {(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)addr),
+                         (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(addr >> 32)) & 0xFFFFu,
+                         (unsigned)__builtin_amdgcn_readfirstlane((int)(steps == 1 ? range_last : range)),
+                         0x00020000u};
+    const int end = KMINOR ? (rows < B ? (int)rows : B) : (steps == 1 ? last_k : BK);
+    sf_lds_load16<J * WAVES * 1024>(rs, lds_wave, along[J] < end ? voff[J] : 0x80000000u);
+  }
+  __device__ __forceinline__ void next() {
+    at += KMINOR ? BK * ld : BK;
+    --steps;
+  }
+
+  // The step into registers, for operands whose chunks are not all aligned and whole.
+  __device__ __forceinline__ void fetch(int wave, int lane) {
+    const int left_k = steps == 1 ? last_k : BK;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int row = (j * WAVES + wave) * RPI + lane / CPR, c = along[j];
+      const long long n = KMINOR ? left_k : rows;                     // rows there are
+      const long long m = (KMINOR ? rows : left_k) - c;               // elements from the chunk on
+      const T *from = at + row * ld + c;
+      sf_u32x4 v = {0, 0, 0, 0};
+      if (row < n && m > 0) {
+        if (m >= V) {
+          v = *reinterpret_cast<const sf_u32x4_any *>(from);
+        } else {
+          typename SfMfma<T>::frag e;
+#pragma unroll
+          for (int i = 0; i < V; ++i) e[i] = i < m ? from[i] : (T)0.0f;
+          v = __builtin_bit_cast(sf_u32x4, e);
+        }
+      }
+      reg[j] = v;
+    }
+    next();
+  }
+
+  __device__ __forceinline__ void store(unsigned char *lds, int wave, int lane) const {
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+      *reinterpret_cast<sf_u32x4 *>(lds + (j * WAVES + wave) * 1024 + lane * 16) = reg[j];
+  }
+
+  // Fragment of the 32 output rows at row0 for the step's s-th 32 bytes of k: this lane's row is
   // row0 + lane % 32, its k are chunk 2 s + lane / 32 of a K-major row.
   static __device__ __forceinline__ frag fragment(const unsigned char *lds, int row0, int s, int lane) {
     const int h = lane >> 5;
     if constexpr (!KMINOR) {
       const int row = row0 + (lane & 31);
-      return *reinterpret_cast<const frag *>(lds + row * 128 + (((2 * s + h) ^ swz(row)) << 4));
+      return *reinterpret_cast<const frag *>(lds + row * STEP + (((2 * s + h) ^ swz(row)) << 4));
     } else if constexpr (S == 4) {
       frag f;
 #pragma unroll
@@ -203,11 +272,13 @@ struct SfOperand {
   }
 };
 
-// The tile's place in a launch of tiles_p x tiles_q x splits workgroups.  Workgroups go to the 8
-// XCDs in turn: each XCD gets one contiguous run of the tiles, so that the operand rows its tiles
-// share stay in its own L2; within a run, 8 tiles along p by all tiles along q.
-__device__ __forceinline__ void sf_tile_of(int b, const SfGemmArgs &a, int *tp, int *tq, int *split) {
-  const int nb = gridDim.x, per = nb >> 3, more = nb & 7, x = b & 7, i = b >> 3;
+// Place of work item b of nb = tiles_p x tiles_q x splits.  Workgroups go to the 8 XCDs in turn (and
+// walk the items in strides of a multiple of 8): each XCD gets one contiguous run of the tiles, so
+// that the operand rows its tiles share stay in its own L2; within a run, 8 tiles along p by all
+// tiles along q.
+__device__ __forceinline__ void sf_tile_of(int b, int nb, const SfGemmArgs &a, int *tp, int *tq,
+                                           int *split) {
+  const int per = nb >> 3, more = nb & 7, x = b & 7, i = b >> 3;
   int t = x * per + (x < more ? x : more) + i;
   const int tiles = a.tiles_p * a.tiles_q;
   *split = t / tiles;
@@ -219,153 +290,389 @@ __device__ __forceinline__ void sf_tile_of(int b, const SfGemmArgs &a, int *tp, 
   *tq = t / high;
 }
 
-template <typename T, bool PMINOR, bool QMINOR, int BP, int BQ, int WP, int WQ, bool DMA, int MINB>
-__global__ void __launch_bounds__(WP *WQ * 64, MINB) sf_gemm_kernel(SfGemmArgs a) {
-  constexpr int WAVES = WP * WQ, V = 16 / sizeof(T), BK = 128 / sizeof(T);
-  constexpr int TP = BP / WP / 32, TQ = BQ / WQ / 32, WTQ = BQ / WQ;
-  constexpr bool kReadFirst = sizeof(T) == 2 && (PMINOR || QMINOR);
-  typedef SfOperand<T, PMINOR, BP, WAVES, DMA> OP;
-  typedef SfOperand<T, QMINOR, BQ, WAVES, DMA> OQ;
+// Steps of a tile's contraction.
+template <int BK>
+__device__ __forceinline__ int sf_steps(const SfGemmArgs &a, int split) {
+  const long long first = split * a.k_split;
+  const long long n = first + a.k_split < a.nk ? a.k_split : a.nk - first;
+  return (int)((n + BK - 1) / BK);
+}
+
+// Epilogue of a wave's TP x TQ blocks of 32 x 32 at (p0, q0).  A block goes through the wave's own
+// 4 KB of LDS (quads of columns swizzled by the row) so that bias, pre, residual and output move in
+// whole 16-byte chunks of a row; the plain sums when the contraction is split.  Stripes of 32 rows are
+// a real loop (unrolled, the code of a large tile outgrows the instruction cache); the accumulators
+// cannot be indexed by it, so each block is picked by comparison.
+template <typename T, int TP, int TQ>
+struct SfEpilogue {
+  static constexpr int V = 16 / sizeof(T), CPL = 32 / V, RPT = 64 / CPL, ITS = 32 / RPT;
+  const SfGemmArgs &a;
+  float *stage;
+  long long p0, q0;
+  int split, lane;
+
+  __device__ __forceinline__ void put(const sf_f32x16 &c) const {
+    const int h = lane >> 5, row = lane & 31;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<sf_f32x4 *>(stage + row * 32 + (((2 * g + h) ^ row ^ (row >> 3)) & 7) * 4) =
+          (sf_f32x4){c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
+  }
+  static __device__ __forceinline__ void meet() {      // the wave's writes before its reads, and back
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  // this lane's chunk of row r (0..31) of the staged block
+  __device__ __forceinline__ void get(int r, float *v) const {
+    const int cl = lane % CPL;
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const int quad = ((cl * V + j) / 4 ^ r ^ (r >> 3)) & 7;
+      const sf_f32x4 f = *reinterpret_cast<const sf_f32x4 *>(stage + r * 32 + quad * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j + e] = f[e];
+    }
+  }
+  __device__ __forceinline__ long long row_of(int t, int it) const {
+    return p0 + t * 32 + it * RPT + lane / CPL;
+  }
+  typedef typename SfChunk<T>::type chunk;
+  typedef SfChunk<float>::type chunk4;
+
+  // All rows and columns of the wave's blocks exist: straight-line code, so that nothing waits for
+  // stores (their vmcnt is shared with the loads) and the residual comes a stripe of 32 rows ahead.
+  struct Ahead {
+    chunk r[2][TQ][ITS];
+  };
+  __device__ __forceinline__ void prefetch(Ahead &n, int t) const {
+    const T *res = static_cast<const T *>(a.residual) + q0 + (lane % CPL) * V;
+#pragma unroll
+    for (int it = 0; it < ITS; ++it)
+#pragma unroll
+      for (int u = 0; u < TQ; ++u)
+        n.r[t & 1][u][it] = *reinterpret_cast<const chunk *>(res + row_of(t, it) * a.nq + u * 32);
+  }
+  __device__ __forceinline__ void sums(const sf_f32x16 (&acc)[TP][TQ]) const {
+#pragma unroll
+    for (int t = 0; t < TP; ++t)
+#pragma unroll
+      for (int u = 0; u < TQ; ++u) {
+        put(acc[t][u]);
+        meet();
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          float v[V];
+          get(it * RPT + lane / CPL, v);
+          float *part = a.partial + ((long long)split * a.np + row_of(t, it)) * a.nq + q0 +
+                        (lane % CPL) * V + u * 32;
+#pragma unroll
+          for (int j = 0; j < V; j += 4)
+            *reinterpret_cast<chunk4 *>(part + j) = (chunk4){v[j], v[j + 1], v[j + 2], v[j + 3]};
+        }
+        meet();
+      }
+  }
+  template <bool RES>
+  __device__ __forceinline__ void whole(const sf_f32x16 (&acc)[TP][TQ], Ahead &ahead) const {
+    const long long col = q0 + (lane % CPL) * V;
+    T *out = static_cast<T *>(a.out) + col, *pre = static_cast<T *>(a.pre);
+    if (pre) pre += col;
+    chunk b[TQ];
+#pragma unroll
+    for (int u = 0; u < TQ; ++u) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) b[u][j] = (T)0.0f;
+      if (a.bias) b[u] = *reinterpret_cast<const chunk *>(static_cast<const T *>(a.bias) + col + u * 32);
+    }
+#pragma unroll
+    for (int t = 0; t < TP; ++t) {
+      if constexpr (RES)
+        if (t + 1 < TP) prefetch(ahead, t + 1);
+#pragma unroll
+      for (int u = 0; u < TQ; ++u) {
+        put(acc[t][u]);
+        meet();
+        float v[ITS][V];
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) get(it * RPT + lane / CPL, v[it]);
+        meet();
+#pragma unroll
+        for (int it = 0; it < ITS; ++it) {
+          const long long at = row_of(t, it) * a.nq + u * 32;
+          chunk c;
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[it][j] += (float)b[u][j];
+          if (pre) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) c[j] = (T)v[it][j];
+            *reinterpret_cast<chunk *>(pre + at) = c;
+          }
+          if (a.act == SF_ACT_GELU) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[it][j] = sf_act<T>(v[it][j], SF_ACT_GELU);
+          } else if (a.act == SF_ACT_RELU) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[it][j] = sf_act<T>(v[it][j], SF_ACT_RELU);
+          }
+          if constexpr (RES) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[it][j] += (float)ahead.r[t & 1][u][it][j];
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) c[j] = (T)v[it][j];
+          *reinterpret_cast<chunk *>(out + at) = c;
+        }
+      }
+    }
+  }
+
+  // Some rows or columns are past the end: element by element where a chunk is cut.  Blocks are a real
+  // loop; the accumulators cannot be indexed by it, so each is picked by comparison.
+  __device__ __forceinline__ void ragged(const sf_f32x16 (&acc)[TP][TQ]) const {
+    const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
+    T *out = static_cast<T *>(a.out), *pre = static_cast<T *>(a.pre);
+#pragma unroll 1
+    for (int tu = 0; tu < TP * TQ; ++tu) {
+      const int t = tu / TQ, u = tu % TQ;
+      if (p0 + t * 32 >= a.np || q0 + u * 32 >= a.nq) continue;
+      const long long col = q0 + u * 32 + (lane % CPL) * V;
+      float w[ITS][V], b[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) b[j] = 0.0f;
+      if (bias && a.splits == 1 && col < a.nq) sf_load_chunk<T>(bias, col, a.nq, b);
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const long long row = row_of(t, it);
+#pragma unroll
+        for (int j = 0; j < V; ++j) w[it][j] = 0.0f;
+        if (res && a.splits == 1 && row < a.np && col < a.nq)
+          sf_load_chunk<T>(res + row * a.nq, col, a.nq, w[it]);
+      }
+#pragma unroll
+      for (int i = 0; i < TP * TQ; ++i)
+        if (tu == i) put(acc[i / TQ][i % TQ]);
+      meet();
+#pragma unroll
+      for (int it = 0; it < ITS; ++it) {
+        const long long row = row_of(t, it);
+        if (row >= a.np || col >= a.nq) continue;
+        float v[V];
+        get(it * RPT + lane / CPL, v);
+        const long long at = row * a.nq;
+        if (a.splits > 1) {
+          float *part = a.partial + (long long)split * a.np * a.nq + at;
+#pragma unroll
+          for (int j = 0; j < V; j += 4) sf_store_chunk<float>(part, col + j, a.nq, v + j);
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += b[j];
+        if (pre) sf_store_chunk<T>(pre + at, col, a.nq, v);
+        if (a.act == SF_ACT_GELU) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = sf_act<T>(v[j], SF_ACT_GELU);
+        } else if (a.act == SF_ACT_RELU) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] = sf_act<T>(v[j], SF_ACT_RELU);
+        }
+        if (res) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) v[j] += w[it][j];
+        }
+        sf_store_chunk<T>(out + at, col, a.nq, v);
+      }
+      meet();
+    }
+  }
+};
+
+template <int N> struct SfInt { static constexpr int value = N; };
+template <int I, int N, typename F>
+__device__ __forceinline__ void sf_unroll(F &&f) {
+  if constexpr (I < N) {
+    f(SfInt<I>());
+    sf_unroll<I + 1, N>(static_cast<F &&>(f));
+  }
+}
+
+// Shape of a kernel: BP x BQ outputs by WP x WQ waves, steps of STEP bytes of k in a ring of RING
+// buffers, WGS workgroups to a CU.
+template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_>
+struct SfShape {
+  static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STEP = STEP_, RING = RING_, WGS = WGS_;
+  static constexpr int WAVES = WP * WQ, BYTES = (BP + BQ) * STEP, LDS = RING * BYTES + WAVES * 4096;
+  static_assert(LDS * WGS <= 160 * 1024 && (RING == 2 || RING == 4), "LDS of a CU");
+};
+
+// s_waitcnt vmcnt(N) lgkmcnt(0)
+template <int N>
+__device__ __forceinline__ void sf_wait_loads() {
+  static_assert(N < 64, "vmcnt has 6 bits");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
+}
+
+template <typename T, bool PMINOR, bool QMINOR, typename SH, bool DMA>
+__global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_gemm_kernel(SfGemmArgs a) {
+  constexpr int BP = SH::BP, BQ = SH::BQ, WQ = SH::WQ, WAVES = SH::WAVES, STEP = SH::STEP;
+  constexpr int RING = SH::RING, BYTES = SH::BYTES, BK = STEP / (int)sizeof(T), NS = STEP / 32;
+  constexpr int TP = BP / SH::WP / 32, TQ = BQ / WQ / 32;
+  typedef SfOperand<T, PMINOR, BP, WAVES, STEP, DMA> OP;
+  typedef SfOperand<T, QMINOR, BQ, WAVES, STEP, DMA> OQ;
   typedef typename SfMfma<T>::frag frag;
-  static_assert(WAVES * 32 * WTQ * 4 <= (BP + BQ) * 128, "the epilogue's stage fits one buffer");
-  __shared__ __attribute__((aligned(1024))) unsigned char s0[(BP + BQ) * 128];
-  __shared__ __attribute__((aligned(1024))) unsigned char s1[(BP + BQ) * 128];
+  constexpr int NI = OP::NI + OQ::NI;
+  static_assert(DMA || RING == 2, "loads through registers are one step ahead");
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wp = wave / WQ, wq = wave % WQ;
-  int tp, tq, split;
-  sf_tile_of(blockIdx.x, a, &tp, &tq, &split);
-  const long long p0 = (long long)tp * BP, q0 = (long long)tq * BQ;
-  const long long k_first = split * a.k_split;
-  const long long k_end = k_first + a.k_split < a.nk ? k_first + a.k_split : a.nk;
-  const int steps = (int)((k_end - k_first + BK - 1) / BK);
+  float *stage = reinterpret_cast<float *>(lds + RING * BYTES) + wave * 1024;
+#if defined(__HIP_DEVICE_COMPILE__)
+  const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) unsigned char *)lds;
+#else
+  const unsigned lds0 = 0;
+#endif
+  const int tiles = a.tiles_p * a.tiles_q * a.splits;
 
+  // The loads run ahead of the products, across the tiles of this workgroup: `lt` is the tile being
+  // loaded.  Behind the last one they go on as loads of nothing, so that the counted waits hold.
   OP op;
   OQ oq;
-  op.init(a.p, a.ldp, p0, a.np, a.nk, wave, lane);
-  oq.init(a.q, a.ldq, q0, a.nq, a.nk, wave, lane);
-  sf_f32x16 acc[TP][TQ];
-#pragma unroll
-  for (int i = 0; i < TP; ++i)
-#pragma unroll
-    for (int j = 0; j < TQ; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
-
-  // One step: every wave's loads into `cur` have landed and every wave is done with `nxt` (the
-  // barrier), the next step's loads start, this step multiplies.
-  auto step = [&](unsigned char *cur, unsigned char *nxt, int i) {
-    __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const bool more = i + 1 < steps;
-    frag fp[4][TP], fq[4][TQ];
-    auto read = [&](int s) {
-#pragma unroll
-      for (int t = 0; t < TP; ++t) fp[s][t] = OP::fragment(cur, (wp * TP + t) * 32, s, lane);
-#pragma unroll
-      for (int t = 0; t < TQ; ++t) fq[s][t] = OQ::fragment(cur + BP * 128, (wq * TQ + t) * 32, s, lane);
-    };
-    // the transposing reads are opaque to the compiler's alias analysis: behind the loads they would
-    // wait for them, so they all go first
-    if constexpr (kReadFirst) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) read(s);
-    }
-    if (more) {
-      op.load(k_first + (long long)(i + 1) * BK, nxt, wave);
-      oq.load(k_first + (long long)(i + 1) * BK, nxt + BP * 128, wave);
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if constexpr (!kReadFirst) read(s);
-#pragma unroll
-      for (int t = 0; t < TP; ++t)
-#pragma unroll
-        for (int u = 0; u < TQ; ++u) acc[t][u] = SfMfma<T>::run(fq[s][u], fp[s][t], acc[t][u]);
-    }
-    if (more) {
-      op.store(nxt, wave, lane);
-      oq.store(nxt + BP * 128, wave, lane);
-    }
-    asm volatile("" ::: "memory");
+  op.init(a.ldp, wave, lane);
+  oq.init(a.ldq, wave, lane);
+  int lt = blockIdx.x;
+  auto open = [&]() {
+    int tp, tq, split;
+    sf_tile_of(lt, tiles, a, &tp, &tq, &split);
+    const long long k0 = split * a.k_split;
+    const int steps = sf_steps<BK>(a, split);
+    const long long left = a.nk - k0 - (long long)(steps - 1) * BK;
+    const int last = left < BK ? (int)left : BK;
+    op.open(a.p, (long long)tp * BP, a.np, k0, steps, last);
+    oq.open(a.q, (long long)tq * BQ, a.nq, k0, steps, last);
   };
-  if (steps > 0) {
-    op.load(k_first, s0, wave);
-    oq.load(k_first, s0 + BP * 128, wave);
-    op.store(s0, wave, lane);
-    oq.store(s0 + BP * 128, wave, lane);
-  }
-  int i = 0;
-  for (; i + 1 < steps; i += 2) {
-    step(s0, s1, i);
-    step(s1, s0, i + 1);
-  }
-  if (i < steps) step(s0, s1, i);
-
-  // Epilogue, 32 rows of the wave's tile at a time: the accumulators go through LDS (quads swizzled
-  // by the row) so that residual and output move in whole 16-byte chunks of a row.
-  __syncthreads();
-  constexpr int QUADS = WTQ / 4, CPL = WTQ / V, RPT = 64 / CPL;
-  float *stage = reinterpret_cast<float *>(s0) + wave * 32 * WTQ;
-  const int cl = lane % CPL, rl = lane / CPL;
-  const long long col = q0 + wq * WTQ + cl * V;
-  const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
-  T *out = static_cast<T *>(a.out), *pre = static_cast<T *>(a.pre);
-  float bv[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) bv[j] = 0.0f;
-  if (bias && a.splits == 1 && col < a.nq) sf_load_chunk<T>(bias, col, a.nq, bv);
-#pragma unroll
-  for (int t = 0; t < TP; ++t) {
-    const int row = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int u = 0; u < TQ; ++u)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int quad = (u * 8 + 2 * g + h) ^ (row & (QUADS - 1));
-        *reinterpret_cast<sf_f32x4 *>(stage + row * WTQ + quad * 4) =
-            (sf_f32x4){acc[t][u][4 * g], acc[t][u][4 * g + 1], acc[t][u][4 * g + 2],
-                       acc[t][u][4 * g + 3]};
-      }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-    for (int r = 0; r < 32; r += RPT) {
-      float v[V];
-#pragma unroll
-      for (int j = 0; j < V; j += 4) {
-        const int quad = ((cl * V + j) / 4) ^ ((r + rl) & (QUADS - 1));
-        const sf_f32x4 f = *reinterpret_cast<const sf_f32x4 *>(stage + (r + rl) * WTQ + quad * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[j + e] = f[e];
-      }
-      const long long prow = p0 + (wp * TP + t) * 32 + r + rl;
-      if (prow >= a.np || col >= a.nq) continue;
-      const long long at = prow * a.nq;
-      if (a.splits > 1) {
-        float *part = a.partial + ((long long)split * a.np + prow) * a.nq;
-#pragma unroll
-        for (int j = 0; j < V; j += 4) sf_store_chunk<float>(part, col + j, a.nq, v + j);
-        continue;
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += bv[j];
-      if (pre) sf_store_chunk<T>(pre + at, col, a.nq, v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = sf_act(v[j], a.act);
-      if (res) {
-        float u[V];
-        sf_load_chunk<T>(res + at, col, a.nq, u);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += u[j];
-      }
-      sf_store_chunk<T>(out + at, col, a.nq, v);
+  auto advance = [&]() {      // behind the last instruction of a step's load
+    if constexpr (DMA) op.next(), oq.next();
+    if (op.steps == 0) {
+      lt += gridDim.x;
+      if (lt < tiles) open();
+      else op.close(), oq.close();
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  // instructions [FROM, TO) of the load of a step into the buffer at `buf`
+  const unsigned lds_wave = lds0 + wave * 1024;
+  auto issue = [&](auto from, auto to, int buf) {
+    sf_unroll<decltype(from)::value, decltype(to)::value>([&](auto j) {
+      constexpr int J = decltype(j)::value;
+      if constexpr (J < OP::NI) op.template issue<J>(lds_wave + buf);
+      else oq.template issue<J - OP::NI>(lds_wave + buf + BP * STEP);
+    });
+  };
+  auto read_one = [&](frag (&fp)[TP], frag (&fq)[TQ], int buf, int s, int r) {
+    // in the order in which the products need them: p0, q0, q1, .., p1, ..
+    if (r == 0) fp[0] = OP::fragment(lds + buf, wp * TP * 32, s, lane);
+    else if (r <= TQ) fq[r - 1] = OQ::fragment(lds + buf + BP * STEP, (wq * TQ + r - 1) * 32, s, lane);
+    else fp[r - TQ] = OP::fragment(lds + buf, (wp * TP + r - TQ) * 32, s, lane);
+  };
+
+  sf_f32x16 acc[TP][TQ];
+  frag fp[2][TP], fq[2][TQ];
+  constexpr int M = TP * TQ, R = TP + TQ, HALF = RING == 2 ? NI : NI / 2;
+  // The products of 32 bytes of k, fragments in set `s`; between them the reads of the following 32
+  // bytes (part rs of the buffer at rbuf, into the other set) and, evenly, `count` instructions of a
+  // load from `from` on.  A wave issues in order and the matrix unit is busy for 32 cycles a product
+  // (64 for fp32): what is not spread between the products holds them up.
+  auto multiply = [&](auto set, int rbuf, int rs, auto from, auto count, int lbuf) {
+    constexpr int SET = decltype(set)::value, FROM = decltype(from)::value, N = decltype(count)::value;
+    sf_unroll<0, M>([&](auto mm) {
+      constexpr int m = decltype(mm)::value, t = m / TQ, u = m % TQ;
+      __builtin_amdgcn_sched_barrier(0);
+      acc[t][u] = SfMfma<T>::run(fq[SET][u], fp[SET][t], acc[t][u]);
+#pragma unroll
+      for (int r = m * R / M; r < (m + 1) * R / M; ++r) read_one(fp[1 - SET], fq[1 - SET], rbuf, rs, r);
+      if constexpr (DMA)
+        issue(SfInt<FROM + m * N / M>(), SfInt<FROM + (m + 1) * N / M>(), lbuf);
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  int cur = 0, last = (RING - 1) * BYTES;      // last: the buffer whose load is half issued
+  open();
+  if constexpr (DMA) {
+#pragma unroll
+    for (int i = 0; i + 1 < RING; ++i) {
+      issue(SfInt<0>(), SfInt<NI>(), i * BYTES);
+      advance();
+    }
+    issue(SfInt<0>(), SfInt<HALF>(), last);
+    sf_wait_loads<(RING - 2) * NI + HALF>();
+  } else {
+    op.fetch(wave, lane), oq.fetch(wave, lane);
+    op.store(lds, wave, lane), oq.store(lds + BP * STEP, wave, lane);
+    advance();
+    if (lt < tiles) op.fetch(wave, lane), oq.fetch(wave, lane);
+    sf_wait_loads<0>();
   }
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    int tp, tq, split;
+    sf_tile_of(tile, tiles, a, &tp, &tq, &split);
+    const int steps = sf_steps<BK>(a, split);
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+#pragma unroll
+      for (int j = 0; j < TQ; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) read_one(fp[0], fq[0], cur, 0, r);      // visible since the last barrier
+    const long long p0 = (long long)tp * BP + wp * TP * 32, q0 = (long long)tq * BQ + wq * TQ * 32;
+    // the epilogue's addresses are not worth registers in the main loop: keep them from being hoisted
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const SfEpilogue<T, TP, TQ> epilogue{a, stage, p0, q0, split, l};
+    typename SfEpilogue<T, TP, TQ>::Ahead ahead;
+    const bool inside = q0 + TQ * 32 <= a.nq && p0 + TP * 32 <= a.np;
+    const bool residual = a.residual && a.splits == 1;
+    // A step: the fragments of each 32 bytes of k are read while the 32 before multiply, and the
+    // second half of the youngest load is issued.  Ahead of the last products the next step has landed
+    // (every wave waits for its own loads, the barrier joins them) and nobody needs this step's buffer
+    // any more: the next step's first fragments and the first half of the load into the freed buffer
+    // run under them.
+    for (int i = 0; i < steps; ++i) {
+      const int nxt = cur + BYTES == RING * BYTES ? 0 : cur + BYTES;
+      multiply(SfInt<0>(), cur, 1, SfInt<HALF>(), SfInt<NI - HALF>(), last);
+#pragma unroll
+      for (int s = 1; s + 2 < NS; s += 2) {
+        multiply(SfInt<1>(), cur, s + 1, SfInt<0>(), SfInt<0>(), 0);
+        multiply(SfInt<0>(), cur, s + 2, SfInt<0>(), SfInt<0>(), 0);
+      }
+      if constexpr (DMA) {
+        advance();
+        asm volatile("" ::: "memory");
+        sf_wait_loads<(RING - 2) * NI>();
+      } else {
+        op.store(lds + nxt, wave, lane), oq.store(lds + nxt + BP * STEP, wave, lane);
+        asm volatile("" ::: "memory");
+        sf_wait_loads<0>();
+      }
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if constexpr (!DMA) {
+        advance();
+        if (lt < tiles) op.fetch(wave, lane), oq.fetch(wave, lane);
+      }
+      if (i + 1 == steps && inside && residual) epilogue.prefetch(ahead, 0);
+      multiply(SfInt<1>(), nxt, 0, SfInt<0>(), SfInt<HALF>(), cur);
+      last = cur;
+      cur = nxt;
+    }
+    if (!inside) epilogue.ragged(acc);
+    else if (a.splits > 1) epilogue.sums(acc);
+    else if (residual) epilogue.template whole<true>(acc, ahead);
+    else epilogue.template whole<false>(acc, ahead);
+  }
+  sf_wait_loads<0>();      // the loads of nothing still write zeros into this workgroup's LDS
 }
 
 // Adds the splits' partial sums in order and applies the epilogue; rows of one chunk a lane.
@@ -393,7 +700,7 @@ __global__ void __launch_bounds__(256) sf_gemm_join_kernel(SfGemmArgs a) {
     }
     if (a.pre) sf_store_chunk<T>(static_cast<T *>(a.pre) + at, col, a.nq, v);
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = sf_act(v[j], a.act);
+    for (int j = 0; j < V; ++j) v[j] = sf_act<T>(v[j], a.act);
     if (a.residual) {
       sf_load_chunk<T>(static_cast<const T *>(a.residual) + at, col, a.nq, u);
 #pragma unroll
@@ -403,35 +710,57 @@ __global__ void __launch_bounds__(256) sf_gemm_join_kernel(SfGemmArgs a) {
   }
 }
 
+template <typename T>
+static void sf_gemm_join(const SfGemmArgs &a, hipStream_t st) {
+  const long long cpr = (a.nq + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T));
+  hipLaunchKernelGGL((sf_gemm_join_kernel<T>), dim3(sf_grid(a.np * cpr, 256)), dim3(256), 0, st, a);
+}
+
 // The launches of one storage type (linear_f32.hip, linear_f16.hip, linear_bf16.hip).
 // layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.
-void sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
-void sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
-void sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
+int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
+int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
+int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
+
+template <typename T, bool PMINOR, bool QMINOR, typename SH, bool DMA>
+static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
+  static SfSlotCache cache;
+  auto kern = sf_gemm_kernel<T, PMINOR, QMINOR, SH, DMA>;
+  int slots = sf_resident_slots(cache, kern, SH::WAVES * 64, 0, SH::LDS);
+  if (slots < 8) {
+    sf_set_error("no occupancy for the matrix product kernel on this device");
+    return SF_ERR_HIP;
+  }
+  slots &= ~7;
+  const long long items = (long long)a.tiles_p * a.tiles_q * a.splits;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items < slots ? items : slots)), dim3(SH::WAVES * 64), 0, st,
+                     a);
+  return SF_OK;
+}
+
+typedef SfShape<256, 256, 2, 4, 64, 4, 1> SfTile256;
+typedef SfShape<128, 128, 2, 2, 128, 2, 2> SfTile128;
+typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64;
 
 template <typename T, bool PMINOR, bool QMINOR>
-static void sf_gemm_launch(const SfGemmArgs &a, int tile, bool dma, hipStream_t st) {
-  const dim3 grid((unsigned)(a.tiles_p * a.tiles_q * a.splits));
-#define SF_GO(B, D, MINB)                                                                          \
-  hipLaunchKernelGGL((sf_gemm_kernel<T, PMINOR, QMINOR, B, B, 2, 2, D, MINB>), grid, dim3(256), 0, \
-                     st, a)
-  if (tile == 128) {
-    if (dma) SF_GO(128, true, 2);
-    else SF_GO(128, false, 2);
-  } else {
-    if (dma) SF_GO(64, true, 4);
-    else SF_GO(64, false, 4);
-  }
-#undef SF_GO
-  if (a.splits > 1) {
-    const long long cpr = (a.nq + 16 / (int)sizeof(T) - 1) / (16 / (int)sizeof(T));
-    hipLaunchKernelGGL((sf_gemm_join_kernel<T>), dim3(sf_grid(a.np * cpr, 256)), dim3(256), 0, st, a);
-  }
+static int sf_gemm_launch(const SfGemmArgs &a, int tile, bool dma, hipStream_t st) {
+  int rc;
+  if (tile == 256 && dma)
+    rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256, true>(a, st);
+  else if (tile == 128)
+    rc = dma ? sf_gemm_go<T, PMINOR, QMINOR, SfTile128, true>(a, st)
+             : sf_gemm_go<T, PMINOR, QMINOR, SfTile128, false>(a, st);
+  else
+    rc = dma ? sf_gemm_go<T, PMINOR, QMINOR, SfTile64, true>(a, st)
+             : sf_gemm_go<T, PMINOR, QMINOR, SfTile64, false>(a, st);
+  if (rc) return rc;
+  if (a.splits > 1) sf_gemm_join<T>(a, st);
+  return SF_OK;
 }
 
 template <typename T>
-static void sf_gemm_any(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st) {
-  if (layout == 0) sf_gemm_launch<T, false, false>(a, tile, dma, st);
-  else if (layout == 1) sf_gemm_launch<T, false, true>(a, tile, dma, st);
-  else sf_gemm_launch<T, true, true>(a, tile, dma, st);
+static int sf_gemm_any(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st) {
+  if (layout == 0) return sf_gemm_launch<T, false, false>(a, tile, dma, st);
+  if (layout == 1) return sf_gemm_launch<T, false, true>(a, tile, dma, st);
+  return sf_gemm_launch<T, true, true>(a, tile, dma, st);
 }

@@ -11,26 +11,32 @@ struct Plan {
   long long k_split;
 };
 
-// Tile and splits of a np x nq product over nk.  128 x 128 tiles once they fill half of the CUs;
-// else 64 x 64, four times as many.  A long contraction with few tiles is cut until there are two
-// workgroups per CU, each at least 4 steps long; the parts are added by sf_gemm_join_kernel.
+// Tile and splits of a np x nq product over nk: the cheapest of the three tiles, each with the splits
+// of a long contraction that would fill the chip, by a model of the busiest CU.
 Plan make_plan(long long np, long long nq, long long nk, int dtype) {
   const long long bk = 128 / (long long)sf_dtype_size(dtype);
   const long long steps = (nk + bk - 1) / bk;
-  auto tiles = [&](long long b) { return ((np + b - 1) / b) * ((nq + b - 1) / b); };
-  Plan pl{128, 1, steps * bk};
-  if (tiles(128) < 128 && (np <= 64 || nq <= 64 || tiles(128) * (steps / 4) < 128)) pl.tile = 64;
-  const long long t = tiles(pl.tile);
-  if (t < 256 && steps >= 8) {
-    long long s = (512 + t - 1) / t;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 1) {
+  Plan best{128, 1, steps * bk};
+  if (np < 1 || nq < 1 || nk < 1) return best;      // no product
+  double least = 1e30;
+  for (int tile : {256, 128, 64}) {
+    const long long t = ((np + tile - 1) / tile) * ((nq + tile - 1) / tile);
+    for (int full = 0; full < 2; ++full) {
+      const int slots = 256 * (tile == 256 ? 1 : tile == 128 ? 2 : 3);
+      long long s = full ? slots / t : 1;
+      if (s > steps / 4) s = steps / 4;
+      if (s < 1 || (full && s == 1)) continue;
       const long long per = (steps + s - 1) / s;
-      pl.splits = (int)((steps + per - 1) / per);
-      pl.k_split = per * bk;
+      s = (steps + per - 1) / per;
+      const double n = (double)((t * s + 255) / 256);
+      double c = dtype == SF_DTYPE_F32
+                     ? n * (tile == 256 ? 8 + 7.9 * per : tile == 128 ? 2 + 2.05 * per : 0.7 + 0.55 * per)
+                     : n * (tile == 256 ? 8 + 1.5 * per : tile == 128 ? 2 + 0.48 * per : 0.8 + 0.21 * per);
+      if (s > 1) c += 3 + 8e-6 * (double)(np * nq * s) / 4.5;
+      if (c < least) least = c, best = Plan{tile, (int)s, per * bk};
     }
   }
-  return pl;
+  return best;
 }
 
 size_t partial_bytes(const Plan &pl, long long np, long long nq) {
@@ -46,18 +52,29 @@ bool direct(const void *p, long long ld, long long extent, int dtype) {
 }
 
 int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st) {
-  const long long tp = (a.np + pl.tile - 1) / pl.tile, tq = (a.nq + pl.tile - 1) / pl.tile;
+  a.splits = pl.splits;
+  a.k_split = pl.k_split;
+  if (a.nk == 0) {      // nothing to sum: the epilogue alone
+    a.splits = 0;
+    if (dtype == SF_DTYPE_F32) sf_gemm_join<float>(a, st);
+    else if (dtype == SF_DTYPE_F16) sf_gemm_join<_Float16>(a, st);
+    else sf_gemm_join<__bf16>(a, st);
+    SF_CHECK_LAUNCH();
+    return SF_OK;
+  }
+  const bool dma = direct(a.p, a.ldp, layout == 2 ? a.np : a.nk, dtype) &&
+                   direct(a.q, a.ldq, layout == 0 ? a.nk : a.nq, dtype);
+  const int tile = !dma && pl.tile > 128 ? 128 : pl.tile;      // no 256 tile through registers
+  const long long tp = (a.np + tile - 1) / tile, tq = (a.nq + tile - 1) / tile;
   SF_CHECK_ARG(tp * tq * pl.splits < SF_INT_MAX, "linear: %lld x %lld outputs are too many for one launch",
                a.np, a.nq);
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  a.splits = pl.splits;
-  a.k_split = pl.k_split;
-  const bool dma = direct(a.p, a.ldp, layout == 2 ? a.np : a.nk, dtype) &&
-                   direct(a.q, a.ldq, layout == 0 ? a.nk : a.nq, dtype);
-  if (dtype == SF_DTYPE_F32) sf_gemm_f32(a, layout, pl.tile, dma, st);
-  else if (dtype == SF_DTYPE_F16) sf_gemm_f16(a, layout, pl.tile, dma, st);
-  else sf_gemm_bf16(a, layout, pl.tile, dma, st);
+  int rc;
+  if (dtype == SF_DTYPE_F32) rc = sf_gemm_f32(a, layout, tile, dma, st);
+  else if (dtype == SF_DTYPE_F16) rc = sf_gemm_f16(a, layout, tile, dma, st);
+  else rc = sf_gemm_bf16(a, layout, tile, dma, st);
+  if (rc) return rc;
   SF_CHECK_LAUNCH();
   return SF_OK;
 }
@@ -85,7 +102,7 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
       if (act != SF_ACT_NONE) {
         sf_load_chunk<T>(pre + r * n, col, n, z);
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[j] *= sf_act_slope(z[j], act);
+        for (int j = 0; j < V; ++j) g[j] *= sf_act_slope<T>(z[j], act);
         if (dz) sf_store_chunk<T>(dz + r * n, col, n, g);
       }
 #pragma unroll
