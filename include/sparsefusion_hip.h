@@ -499,6 +499,9 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
 #define SF_ACT_RELU 1
 #define SF_ACT_GELU 2 /* z/2 (1 + erf(z / sqrt(2))) */
 
+/* Most features, in or out (a tile's rows stay in reach of 31-bit offsets). */
+#define SF_LINEAR_MOST_FEATURES (1 << 20)
+
 /* Bytes of scratch sf_linear needs (0 for most sizes). */
 SF_API size_t sf_linear_workspace(long long m, long long k, long long n, int dtype);
 

@@ -9,6 +9,7 @@ import subprocess
 
 import torch
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libsparsefusion_hip.so')
 _LIB = None
@@ -169,7 +170,10 @@ def ptr(t):
 
 
 def stream(device=None):
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the current stream of `device` (2 us less than torch.cuda.current_stream, which makes
+    an object of it; a call of a small operator takes 8)."""
+    index = None if device is None else device.index
+    return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
 def require(t, dtype, what):
@@ -182,61 +186,47 @@ def require(t, dtype, what):
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-class _Here:
-    """Context of a call whose device is the current one already."""
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        pass
-
-
-_HERE_ALREADY = _Here()
-
-
-def on(device):
-    """Context in which `device` is the current one: kernels launch, and outputs and scratch are
-    allocated, on the tensors' own device."""
+def elsewhere(device):
+    """Whether `device` is another one than the current: then the caller enters torch.cuda.device, so
+    that kernels launch, and outputs and scratch are allocated, on the tensors' own device."""
     if device.type != 'cuda':
         raise RuntimeError('sparsefusion_amd ops need tensors on a HIP device '
                            f'(got {device}); there is no CPU path')
-    if device.index == torch.cuda.current_device():
-        return _HERE_ALREADY
-    return torch.cuda.device(device)
+    return device.index != torch.cuda.current_device()
 
 
-def same(x, **others):
-    """Refuse tensors of another type or on another device than x."""
-    for name, t in others.items():
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise RuntimeError(f'{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}')
+def same(x, name, t):
+    """Refuse a tensor of another type or on another device than x."""
+    if t.dtype != x.dtype or t.device != x.device:
+        raise RuntimeError(f'{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}')
 
 
 def rows(x):
     """(..., K) as (M, K) with adjacent elements and evenly spaced rows, and their distance; a copy
     only where the strides do not allow a view."""
     k = x.shape[-1]
+    if x.dim() == 2 and x.is_contiguous():
+        return x, k
     flat = x.reshape(x.numel() // k if k else x.shape[:-1].numel(), k)
     if k > 1 and flat.stride(1) != 1 or flat.shape[0] > 1 and flat.stride(0) < k:
         flat = flat.contiguous()
     return flat, flat.stride(0) if flat.shape[0] > 1 else k
 
 
-def dev_ptr(t):
-    """ptr() for a tensor whose row distance is handed over with it."""
-    if not t.is_cuda:
-        return ptr(t)
-    return t.data_ptr()
+def workspace(nbytes, x):
+    """Scratch memory beside x from the caching allocator, None for none.  The block returns to the
+    current stream's pool when the caller drops it and is handed out again in that stream's order only;
+    under capture it belongs to the graph's own pool."""
+    return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
-def workspace(nbytes, device):
-    """(tensor, size) of scratch memory from the caching allocator, (None, 0) for none.  The block
-    returns to the current stream's pool when the caller drops it and is handed out again in that
-    stream's order only; under capture it belongs to the graph's own pool."""
-    if not nbytes:
-        return None, 0
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+def differentiable(*tensors):
+    """Whether autograd would record an operation on these tensors."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class _ForwardOnly(torch.autograd.Function):

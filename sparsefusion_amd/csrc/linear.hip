@@ -199,7 +199,7 @@ BackwardPlan backward_plan(long long m, long long k, long long n, int dtype, int
 
 bool good_sizes(long long m, long long k, long long n, int dtype) {
   return m >= 0 && k >= 0 && n >= 0 && dtype >= SF_DTYPE_F32 && dtype <= SF_DTYPE_BF16 &&
-         m < (1LL << 40) && k < SF_INT_MAX && n < SF_INT_MAX;
+         m < (1LL << 40) && k <= SF_LINEAR_MOST_FEATURES && n <= SF_LINEAR_MOST_FEATURES;
 }
 
 #define SF_LINEAR_CHECK()                                                                          \

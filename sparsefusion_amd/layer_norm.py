@@ -15,24 +15,27 @@ from .registry import NORM_LAYERS
 
 
 def _check(x, weight, bias):
-    if x.dtype not in _lib.DTYPE_CODES:
-        raise RuntimeError(f'layer_norm takes fp32, fp16 or bf16, got {x.dtype}')
+    """-> (d, dtype code, parameters' type) of well-formed rows and parameters."""
+    dtype = x.dtype
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None:
+        raise RuntimeError(f'layer_norm takes fp32, fp16 or bf16, got {dtype}')
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f'layer_norm needs rows of at least one element, got {tuple(x.shape)}')
     d = x.shape[-1]
-    dtype = None
+    pdtype = None
     for name, t in (('weight', weight), ('bias', bias)):
         if t is None:
             continue
-        if tuple(t.shape) != (d,):
+        if t.dim() != 1 or t.shape[0] != d:
             raise RuntimeError(f'{name} must have shape ({d},), got {tuple(t.shape)}')
         if t.device != x.device:
             raise RuntimeError(f'{name} is on {t.device}, x on {x.device}')
-        if t.dtype not in (x.dtype, torch.float32) or t.dtype != (dtype or t.dtype):
-            raise RuntimeError(f'weight and bias must both be {x.dtype} or both float32, '
+        if t.dtype not in (dtype, torch.float32) or t.dtype != (pdtype or t.dtype):
+            raise RuntimeError(f'weight and bias must both be {dtype} or both float32, '
                                f'{name} is {t.dtype}')
-        dtype = t.dtype
-    return dtype or x.dtype
+        pdtype = t.dtype
+    return d, code, pdtype or dtype
 
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=False,
@@ -40,29 +43,36 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, retur
     """-> (y, sum, mean, rstd) of s = x + residual, y = (s - mean) * rstd * weight + bias.  sum (s
     rounded) with return_sum, mean and rstd (fp32, x.shape[:-1]) with keep_stats, else None.  Not
     differentiable: see `layer_norm`."""
-    pdtype = _check(x, weight, bias)
+    d, code, pdtype = _check(x, weight, bias)
     if not eps >= 0:
         raise RuntimeError(f'eps must not be negative, got {eps}')
-    d = x.shape[-1]
     if residual is not None:
-        _lib.same(x, residual=residual)
+        _lib.same(x, 'residual', residual)
         if residual.shape != x.shape:
             residual = residual.expand(x.shape)
         residual = residual.contiguous()
+    if _lib.elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return layer_norm_forward(x, weight, bias, eps, residual, return_sum, keep_stats)
     x = x.contiguous()
-    m = x.numel() // d
-    with _lib.on(x.device):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if return_sum else None
-        mean = rstd = None
-        if keep_stats:
-            mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-            rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        _lib.check(_lib.lib().sf_layer_norm(
-            _lib.ptr(x), _lib.ptr(residual), _lib.ptr(weight.contiguous()) if weight is not None else None,
-            _lib.ptr(bias.contiguous()) if bias is not None else None, y.data_ptr(), _lib.ptr(s),
-            _lib.ptr(mean), _lib.ptr(rstd), m, d, eps, _lib.DTYPE_CODES[x.dtype],
-            _lib.DTYPE_CODES[pdtype], _lib.stream(x.device)))
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    y = torch.empty_like(x)
+    s = torch.empty_like(x) if return_sum else None
+    mean = rstd = None
+    if keep_stats:
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rc = _lib.lib().sf_layer_norm(
+        x.data_ptr(), None if residual is None else residual.data_ptr(),
+        None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(),
+        y.data_ptr(), None if s is None else s.data_ptr(), None if mean is None else mean.data_ptr(),
+        None if rstd is None else rstd.data_ptr(), x.numel() // d, d, eps, code,
+        _lib.DTYPE_CODES[pdtype], _lib.stream(x.device))
+    if rc:
+        _lib.check(rc)
     return y, s, mean, rstd
 
 
@@ -72,37 +82,45 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, grad_sum=None, needs=(
     `grad_sum` of the sum (or None); x is the normalised sum, mean and rstd as it returned them.  dx is
     the gradient of x and of the residual alike.  `needs` says which are wanted, the others are None;
     the parameter gradients have weight's type (without a weight: `param_dtype`, or x's)."""
-    pdtype = _check(x, weight, None)
+    d, code, pdtype = _check(x, weight, None)
     if weight is None and param_dtype is not None:
         pdtype = param_dtype
         if pdtype not in (x.dtype, torch.float32):
             raise RuntimeError(f'param_dtype must be {x.dtype} or float32, got {pdtype}')
-    _lib.same(x, grad=grad, grad_sum=grad_sum)
-    d = x.shape[-1]
     for name, t in (('grad', grad), ('grad_sum', grad_sum)):
-        if t is not None and t.shape != x.shape:
-            raise RuntimeError(f'{name} must have shape {tuple(x.shape)}, got {tuple(t.shape)}')
+        if t is not None:
+            _lib.same(x, name, t)
+            if t.shape != x.shape:
+                raise RuntimeError(f'{name} must have shape {tuple(x.shape)}, got {tuple(t.shape)}')
     m = x.numel() // d
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.dtype != torch.float32 or t.numel() != m or t.device != x.device:
             raise RuntimeError(f'{name} must be {m} fp32 values on {x.device}, got {tuple(t.shape)} '
                                f'{t.dtype} on {t.device}')
+    if _lib.elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return layer_norm_backward(grad, x, mean, rstd, weight, grad_sum, needs, param_dtype)
     grad, x = grad.contiguous(), x.contiguous()
-    grad_sum = grad_sum.contiguous() if grad_sum is not None else None
+    if grad_sum is not None:
+        grad_sum = grad_sum.contiguous()
+    if weight is not None:
+        weight = weight.contiguous()
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    with _lib.on(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty((d,), dtype=pdtype, device=x.device) if needs[1] else None
-        db = torch.empty((d,), dtype=pdtype, device=x.device) if needs[2] else None
-        dtype = _lib.DTYPE_CODES[x.dtype]
-        L = _lib.lib()
-        need = L.sf_layer_norm_backward_workspace(m, d, dtype) if needs[1] or needs[2] else 0
-        ws, nbytes = _lib.workspace(need, x.device)
-        _lib.check(L.sf_layer_norm_backward(
-            _lib.ptr(grad), _lib.ptr(x), _lib.ptr(mean), _lib.ptr(rstd),
-            _lib.ptr(weight.contiguous()) if weight is not None else None, _lib.ptr(grad_sum),
-            dx.data_ptr(), _lib.ptr(dw), _lib.ptr(db), m, d, dtype, _lib.DTYPE_CODES[pdtype],
-            _lib.ptr(ws), nbytes, _lib.stream(x.device)))
+    dx = torch.empty_like(x)
+    dw = x.new_empty(d, dtype=pdtype) if needs[1] else None
+    db = x.new_empty(d, dtype=pdtype) if needs[2] else None
+    L = _lib.lib()
+    nbytes = L.sf_layer_norm_backward_workspace(m, d, code) if needs[1] or needs[2] else 0
+    ws = _lib.workspace(nbytes, x)
+    rc = L.sf_layer_norm_backward(
+        grad.data_ptr(), x.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+        None if weight is None else weight.data_ptr(),
+        None if grad_sum is None else grad_sum.data_ptr(), dx.data_ptr(),
+        None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, d, code,
+        _lib.DTYPE_CODES[pdtype], None if ws is None else ws.data_ptr(), nbytes,
+        _lib.stream(x.device))
+    if rc:
+        _lib.check(rc)
     return dx if needs[0] else None, dw, db
 
 
@@ -136,8 +154,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=Fa
     """Layer norm of x + residual over the last dimension, differentiable in all four tensors; with
     return_sum -> (y, sum), for blocks that carry the sum on.  weight and bias (D,) or None; residual
     has x's shape or expands to it (its gradient is summed back)."""
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _lib.differentiable(x, weight, bias, residual):
         if residual is not None and residual.shape != x.shape:
             residual = residual.expand(x.shape)
         return _LayerNorm.apply(x, weight, bias, eps, residual, return_sum)

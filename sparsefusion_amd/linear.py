@@ -14,26 +14,31 @@ from torch import nn
 from . import _lib
 from .registry import LINEAR_LAYERS
 
+MOST_FEATURES = 1 << 20      # in or out: a tile's rows stay in reach of 31-bit offsets
 ACTIVATIONS = {None: 0, 'none': 0, 'relu': 1, 'gelu': 2}
 
 
 def _act_code(activation):
-    if activation not in ACTIVATIONS:
+    code = ACTIVATIONS.get(activation)
+    if code is None:
         raise RuntimeError(f"activation must be None, 'none', 'relu' or 'gelu' (erf), got {activation!r}")
-    return ACTIVATIONS[activation]
+    return code
 
 
-def _check(x, weight, bias):
-    if x.dtype not in _lib.DTYPE_CODES:
+def _check(x, weight):
+    """-> (n, k, dtype code) of a well-formed pair."""
+    code = _lib.DTYPE_CODES.get(x.dtype)
+    if code is None:
         raise RuntimeError(f'linear takes fp32, fp16 or bf16, got {x.dtype}')
     if weight.dim() != 2:
         raise RuntimeError(f'weight must be (out_features, in_features), got {tuple(weight.shape)}')
     n, k = weight.shape
     if x.dim() < 1 or x.shape[-1] != k:
         raise RuntimeError(f'expected rows of {k} elements, got {tuple(x.shape)}')
-    _lib.same(x, weight=weight, bias=bias)
-    if bias is not None and tuple(bias.shape) != (n,):
-        raise RuntimeError(f'bias must have shape ({n},), got {tuple(bias.shape)}')
+    if max(n, k) > MOST_FEATURES:
+        raise RuntimeError(f'linear takes up to {MOST_FEATURES} features, got {k} -> {n}')
+    _lib.same(x, 'weight', weight)
+    return n, k, code
 
 
 def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pre=False):
@@ -41,28 +46,36 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     the activation (None otherwise).  x (..., K), weight (N, K), bias (N,), residual (..., N) or
     anything that expands to it.  Not differentiable: see `linear`."""
     act = _act_code(activation)
-    _check(x, weight, bias)
-    n, k = weight.shape
-    shape = x.shape[:-1] + (n,)
-    rows, ldx = _lib.rows(x)
-    m = rows.shape[0]
+    n, k, code = _check(x, weight)
+    shape = (x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n)
+    if bias is not None:
+        _lib.same(x, 'bias', bias)
+        if bias.dim() != 1 or bias.shape[0] != n:
+            raise RuntimeError(f'bias must have shape ({n},), got {tuple(bias.shape)}')
+        bias = bias.contiguous()
     if residual is not None:
-        _lib.same(x, residual=residual)
+        _lib.same(x, 'residual', residual)
         if residual.shape != shape:
             residual = residual.expand(shape)
         residual = residual.contiguous()
-    w = weight.contiguous()
-    with _lib.on(x.device):
-        y = torch.empty(shape, dtype=x.dtype, device=x.device)
-        pre = torch.empty(shape, dtype=x.dtype, device=x.device) if keep_pre else None
-        dtype = _lib.DTYPE_CODES[x.dtype]
-        L = _lib.lib()
-        ws, nbytes = _lib.workspace(L.sf_linear_workspace(m, k, n, dtype), x.device)
-        _lib.check(L.sf_linear(
-            _lib.dev_ptr(rows), ldx, _lib.ptr(w),
-            _lib.ptr(bias.contiguous()) if bias is not None else None, _lib.ptr(residual),
-            y.data_ptr(), pre.data_ptr() if keep_pre else None, m, k, n, dtype, act, _lib.ptr(ws), nbytes,
-            _lib.stream(x.device)))
+    if _lib.elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return linear_forward(x, weight, bias, activation, residual, keep_pre)
+    rows, ldx = _lib.rows(x)
+    m = rows.shape[0]
+    weight = weight.contiguous()
+    y = x.new_empty(shape)
+    pre = x.new_empty(shape) if keep_pre else None
+    L = _lib.lib()
+    nbytes = L.sf_linear_workspace(m, k, n, code)
+    ws = _lib.workspace(nbytes, x)
+    rc = L.sf_linear(
+        rows.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(),
+        None if residual is None else residual.data_ptr(), y.data_ptr(),
+        None if pre is None else pre.data_ptr(), m, k, n, code, act,
+        None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
+    if rc:
+        _lib.check(rc)
     return y, pre
 
 
@@ -71,29 +84,38 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     output; `pre` as it returned them (not needed without an activation).  `needs` says which are
     wanted, the others are None.  The residual's gradient is `grad` itself."""
     act = _act_code(activation)
-    _check(x, weight, None)
-    n, k = weight.shape
-    shape = x.shape[:-1] + (n,)
-    _lib.same(x, grad=grad, pre=pre if act else None)
-    if act and pre is None:
+    n, k, code = _check(x, weight)
+    shape = (*x.shape[:-1], n)
+    if not act:
+        pre = None
+    elif pre is None:
         raise RuntimeError(f"the gradient of '{activation}' needs the values before it (pre)")
-    for name, t in (('grad', grad), ('pre', pre if act else None)):
-        if t is not None and t.shape != shape:
-            raise RuntimeError(f'{name} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+    for name, t in (('grad', grad), ('pre', pre)):
+        if t is not None:
+            _lib.same(x, name, t)
+            if t.shape != shape:
+                raise RuntimeError(f'{name} must have shape {shape}, got {tuple(t.shape)}')
+    if _lib.elsewhere(x.device):
+        with torch.cuda.device(x.device):
+            return linear_backward(grad, x, weight, pre, activation, needs)
     rows, ldx = _lib.rows(x)
     m = rows.shape[0]
-    grad, w = grad.contiguous(), weight.contiguous()
-    pre = pre.contiguous() if act else None
-    with _lib.on(x.device):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if needs[0] else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if needs[1] else None
-        db = torch.empty((n,), dtype=x.dtype, device=x.device) if needs[2] else None
-        dtype = _lib.DTYPE_CODES[x.dtype]
-        L = _lib.lib()
-        ws, nbytes = _lib.workspace(L.sf_linear_backward_workspace(m, k, n, dtype, act), x.device)
-        _lib.check(L.sf_linear_backward(
-            _lib.ptr(grad), _lib.dev_ptr(rows), ldx, _lib.ptr(w), _lib.ptr(pre), _lib.ptr(dx),
-            _lib.ptr(dw), _lib.ptr(db), m, k, n, dtype, act, _lib.ptr(ws), nbytes, _lib.stream(x.device)))
+    grad, weight = grad.contiguous(), weight.contiguous()
+    if pre is not None:
+        pre = pre.contiguous()
+    dx = x.new_empty(x.shape) if needs[0] else None
+    dw = x.new_empty((n, k)) if needs[1] else None
+    db = x.new_empty(n) if needs[2] else None
+    L = _lib.lib()
+    nbytes = L.sf_linear_backward_workspace(m, k, n, code, act)
+    ws = _lib.workspace(nbytes, x)
+    rc = L.sf_linear_backward(
+        grad.data_ptr(), rows.data_ptr(), ldx, weight.data_ptr(),
+        None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
+        None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code,
+        act, None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
+    if rc:
+        _lib.check(rc)
     return dx, dw, db
 
 
@@ -124,8 +146,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x @ weight.T + bias) + residual, differentiable in all four tensors.  x (..., K), weight
     (N, K), bias (N,); activation None, 'relu' or 'gelu'; residual (..., N) or anything that expands
     to it (its gradient is summed back)."""
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _lib.differentiable(x, weight, bias, residual):
         if residual is not None and x.dim() and residual.shape != x.shape[:-1] + weight.shape[:1]:
             residual = residual.expand(x.shape[:-1] + weight.shape[:1])
         return _Linear.apply(x, weight, bias, activation, residual)

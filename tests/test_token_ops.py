@@ -149,6 +149,7 @@ def test_refusals_need_no_device():
             (lambda: linear(torch.zeros(()), w), 'rows of 8'),
             (lambda: linear(x, w, torch.zeros(5)), r'shape \(6,\)'),
             (lambda: linear(x, w[0]), 'out_features'),
+            (lambda: linear(torch.zeros(1, 1), torch.zeros((1 << 20) + 1, 1)), 'features'),
             (lambda: linear(x, w, activation='tanh'), 'activation'),
             (lambda: Linear(4, 4, activation='swish'), 'activation'),
             (lambda: linear(x, w, residual=torch.zeros(3, 6)), 'expand'),
