@@ -502,10 +502,13 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
 /* Most features, in or out (a tile's rows stay in reach of 31-bit offsets). */
 #define SF_LINEAR_MOST_FEATURES (1 << 20)
 
-/* Bytes of scratch sf_linear needs (0 for most sizes). */
-SF_API size_t sf_linear_workspace(long long m, long long k, long long n, int dtype);
+/* Bytes of scratch (16-byte aligned) sf_linear needs for these operands; 0 for most.  The pointers are
+ * looked at, not followed: operands that are not made of aligned 16-byte pieces are copied first. */
+SF_API size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
+                                  long long k, long long n, int dtype);
 
-/* y = act(x weight^T + bias) + residual, one launch (two when few rows meet a long k).
+/* y = act(x weight^T + bias) + residual, one launch (one more when few rows meet a long k, and one for
+ * operands that have to be copied).
  *   x (m, k), rows ldx >= k elements apart;  weight (n, k);  bias (n) or NULL;
  *   residual (m, n) or NULL;  y (m, n);  pre (m, n) or NULL: the values before the activation, which
  *   sf_linear_backward takes.  All of one dtype.  m, k, n may be 0. */
@@ -513,8 +516,10 @@ SF_API int sf_linear(const void *x, long long ldx, const void *weight, const voi
                      const void *residual, void *y, void *pre, long long m, long long k, long long n,
                      int dtype, int act, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Bytes of scratch sf_linear_backward needs. */
-SF_API size_t sf_linear_backward_workspace(long long m, long long k, long long n, int dtype, int act);
+/* Bytes of scratch (16-byte aligned) sf_linear_backward needs for these operands. */
+SF_API size_t sf_linear_backward_workspace(const void *dy, const void *x, long long ldx,
+                                           const void *weight, long long m, long long k, long long n,
+                                           int dtype, int act);
 
 /* Gradients of sf_linear for the gradient dy (m, n) of y:
  *   dz = dy act'(pre);  dx (m, k) = dz weight;  dw (n, k) = dz^T x;  db (n) = sum of dz's rows.

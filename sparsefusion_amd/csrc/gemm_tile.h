@@ -11,9 +11,8 @@
 //   backward dw = dz^T x    P = dz K-minor   Q = x K-minor
 //
 // A workgroup owns a BP x BQ tile and walks k in steps of 128 bytes (64 16-bit or 32 fp32 elements).
-// Both operands' tiles go to LDS in 16-byte chunks, straight from memory (buffer_load ... lds) when
-// every chunk is aligned and whole, through registers otherwise; two buffers, the loads two steps
-// ahead.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32; Q is the instruction's first
+// Both operands' tiles go to LDS in 16-byte chunks straight from memory (buffer_load ... lds), into a
+// ring of buffers up to three steps ahead.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32; Q is the instruction's first
 // operand, so a lane ends up with four consecutive q of one row p.  Workgroups stay and walk the
 // tiles: the loads of the next tile's first steps run under the epilogue of the last.
 // Rows and k outside the operands read as zeros (the buffer descriptor's range check), columns
@@ -130,7 +129,7 @@ __device__ __forceinline__ void sf_lds_load16(const sf_u32x4 &rs, unsigned lds, 
 
 // One operand's side of the tile: B rows of the output, KMINOR as above, STEP bytes of a row's k (128
 // or 64) brought at a time.
-template <typename T, bool KMINOR, int B, int WAVES, int STEP, bool DMA>
+template <typename T, bool KMINOR, int B, int WAVES, int STEP>
 struct SfOperand {
   static constexpr int S = sizeof(T), V = 16 / S, BK = STEP / S;
   static constexpr int CPR = KMINOR ? B * S / 16 : STEP / 16;     // chunks of one LDS row
@@ -149,13 +148,12 @@ struct SfOperand {
   }
 
   const T *at;              // the step being loaded: the tile's first row / column at its k
-  long long rows;           // output rows this operand has from the tile's first on
+  long long rows;           // output rows this operand has from the tile's first on, whole chunks
   long long ld;
   int steps, last_k;        // steps to go in this tile, k of its last one
-  unsigned range, range_last;       // DMA: bytes from `at` to the last element of a step in use
-  unsigned voff[DMA ? NI : 1];      // DMA: byte offset of this lane's chunk from `at`
+  unsigned range, range_last;       // bytes from `at` to the last element of a step in use
+  unsigned voff[NI];        // byte offset of this lane's chunk from `at`
   int along[NI];            // K-major: the chunk's k; K-minor: its first output row
-  sf_u32x4 reg[DMA ? 1 : NI];
 
   __device__ __forceinline__ void init(long long ld_, int wave, int lane) {
     ld = ld_;
@@ -164,25 +162,25 @@ struct SfOperand {
       const int row = (j * WAVES + wave) * RPI + lane / CPR;
       const int c = (lane % CPR) ^ swz(row);
       along[j] = c * V;
-      if constexpr (DMA) voff[j] = (unsigned)((long long)row * ld * S) + c * 16u;
+      voff[j] = (unsigned)((long long)row * ld * S) + c * 16u;
     }
   }
-  // A tile: output rows `first` on (of `total`), k from k0 on in `steps` steps, the last of last_k.
+  // A tile: output rows `first` on (of `total`), k from k0 on in `steps` steps, the last of last_k.  The
+  // contiguous extent is made of whole chunks (the host repacks an operand whose is not, with zeros
+  // behind); rows past the range read as zeros (all of it fits 31 bits: the host sees to that too).
   __device__ __forceinline__ void open(const void *ptr, long long first, long long total, long long k0,
                                        int steps_, int last_k_) {
-    rows = total - first;
-    steps = steps_, last_k = last_k_;
+    steps = steps_;
     at = static_cast<const T *>(ptr) + (KMINOR ? first + k0 * ld : first * ld + k0);
-    if constexpr (DMA) {
-      // rows past the range read as zeros (the host sees to it that all of this fits 31 bits)
+    if constexpr (KMINOR) {
+      rows = ((total + V - 1) & ~(long long)(V - 1)) - first, last_k = last_k_;
+      range = (unsigned)(((BK - 1) * ld + rows) * S);
+      range_last = (unsigned)(((last_k - 1) * ld + rows) * S);
+    } else {
+      rows = total - first, last_k = (last_k_ + V - 1) & ~(V - 1);
       const int n = rows < B ? (int)rows : B;
-      if constexpr (KMINOR) {
-        range = (unsigned)(((BK - 1) * ld + rows) * S);
-        range_last = (unsigned)(((last_k - 1) * ld + rows) * S);
-      } else {
-        range = (unsigned)(((n - 1) * ld + BK) * S);
-        range_last = (unsigned)(((n - 1) * ld + last_k) * S);
-      }
+      range = (unsigned)(((n - 1) * ld + BK) * S);
+      range_last = (unsigned)(((n - 1) * ld + last_k) * S);
     }
   }
   __device__ __forceinline__ void close() {      // nothing left to load: zeros from here on
@@ -205,37 +203,6 @@ struct SfOperand {
   __device__ __forceinline__ void next() {
     at += KMINOR ? BK * ld : BK;
     --steps;
-  }
-
-  // The step into registers, for operands whose chunks are not all aligned and whole.
-  __device__ __forceinline__ void fetch(int wave, int lane) {
-    const int left_k = steps == 1 ? last_k : BK;
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-      const int row = (j * WAVES + wave) * RPI + lane / CPR, c = along[j];
-      const long long n = KMINOR ? left_k : rows;                     // rows there are
-      const long long m = (KMINOR ? rows : left_k) - c;               // elements from the chunk on
-      const T *from = at + row * ld + c;
-      sf_u32x4 v = {0, 0, 0, 0};
-      if (row < n && m > 0) {
-        if (m >= V) {
-          v = *reinterpret_cast<const sf_u32x4_any *>(from);
-        } else {
-          typename SfMfma<T>::frag e;
-#pragma unroll
-          for (int i = 0; i < V; ++i) e[i] = i < m ? from[i] : (T)0.0f;
-          v = __builtin_bit_cast(sf_u32x4, e);
-        }
-      }
-      reg[j] = v;
-    }
-    next();
-  }
-
-  __device__ __forceinline__ void store(unsigned char *lds, int wave, int lane) const {
-#pragma unroll
-    for (int j = 0; j < NI; ++j)
-      *reinterpret_cast<sf_u32x4 *>(lds + (j * WAVES + wave) * 1024 + lane * 16) = reg[j];
   }
 
   // Fragment of the 32 output rows at row0 for the step's s-th 32 bytes of k: this lane's row is
@@ -512,16 +479,15 @@ __device__ __forceinline__ void sf_wait_loads() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
 }
 
-template <typename T, bool PMINOR, bool QMINOR, typename SH, bool DMA>
+template <typename T, bool PMINOR, bool QMINOR, typename SH>
 __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_gemm_kernel(SfGemmArgs a) {
   constexpr int BP = SH::BP, BQ = SH::BQ, WQ = SH::WQ, WAVES = SH::WAVES, STEP = SH::STEP;
   constexpr int RING = SH::RING, BYTES = SH::BYTES, BK = STEP / (int)sizeof(T), NS = STEP / 32;
   constexpr int TP = BP / SH::WP / 32, TQ = BQ / WQ / 32;
-  typedef SfOperand<T, PMINOR, BP, WAVES, STEP, DMA> OP;
-  typedef SfOperand<T, QMINOR, BQ, WAVES, STEP, DMA> OQ;
+  typedef SfOperand<T, PMINOR, BP, WAVES, STEP> OP;
+  typedef SfOperand<T, QMINOR, BQ, WAVES, STEP> OQ;
   typedef typename SfMfma<T>::frag frag;
   constexpr int NI = OP::NI + OQ::NI;
-  static_assert(DMA || RING == 2, "loads through registers are one step ahead");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wp = wave / WQ, wq = wave % WQ;
@@ -551,7 +517,7 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
     oq.open(a.q, (long long)tq * BQ, a.nq, k0, steps, last);
   };
   auto advance = [&]() {      // behind the last instruction of a step's load
-    if constexpr (DMA) op.next(), oq.next();
+    op.next(), oq.next();
     if (op.steps == 0) {
       lt += gridDim.x;
       if (lt < tiles) open();
@@ -589,29 +555,20 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
       acc[t][u] = SfMfma<T>::run(fq[SET][u], fp[SET][t], acc[t][u]);
 #pragma unroll
       for (int r = m * R / M; r < (m + 1) * R / M; ++r) read_one(fp[1 - SET], fq[1 - SET], rbuf, rs, r);
-      if constexpr (DMA)
-        issue(SfInt<FROM + m * N / M>(), SfInt<FROM + (m + 1) * N / M>(), lbuf);
+      issue(SfInt<FROM + m * N / M>(), SfInt<FROM + (m + 1) * N / M>(), lbuf);
     });
     __builtin_amdgcn_sched_barrier(0);
   };
 
   int cur = 0, last = (RING - 1) * BYTES;      // last: the buffer whose load is half issued
   open();
-  if constexpr (DMA) {
 #pragma unroll
-    for (int i = 0; i + 1 < RING; ++i) {
-      issue(SfInt<0>(), SfInt<NI>(), i * BYTES);
-      advance();
-    }
-    issue(SfInt<0>(), SfInt<HALF>(), last);
-    sf_wait_loads<(RING - 2) * NI + HALF>();
-  } else {
-    op.fetch(wave, lane), oq.fetch(wave, lane);
-    op.store(lds, wave, lane), oq.store(lds + BP * STEP, wave, lane);
+  for (int i = 0; i + 1 < RING; ++i) {
+    issue(SfInt<0>(), SfInt<NI>(), i * BYTES);
     advance();
-    if (lt < tiles) op.fetch(wave, lane), oq.fetch(wave, lane);
-    sf_wait_loads<0>();
   }
+  issue(SfInt<0>(), SfInt<HALF>(), last);
+  sf_wait_loads<(RING - 2) * NI + HALF>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -647,21 +604,11 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
         multiply(SfInt<1>(), cur, s + 1, SfInt<0>(), SfInt<0>(), 0);
         multiply(SfInt<0>(), cur, s + 2, SfInt<0>(), SfInt<0>(), 0);
       }
-      if constexpr (DMA) {
-        advance();
-        asm volatile("" ::: "memory");
-        sf_wait_loads<(RING - 2) * NI>();
-      } else {
-        op.store(lds + nxt, wave, lane), oq.store(lds + nxt + BP * STEP, wave, lane);
-        asm volatile("" ::: "memory");
-        sf_wait_loads<0>();
-      }
+      advance();
+      asm volatile("" ::: "memory");
+      sf_wait_loads<(RING - 2) * NI>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if constexpr (!DMA) {
-        advance();
-        if (lt < tiles) op.fetch(wave, lane), oq.fetch(wave, lane);
-      }
       if (i + 1 == steps && inside && residual) epilogue.prefetch(ahead, 0);
       multiply(SfInt<1>(), nxt, 0, SfInt<0>(), SfInt<HALF>(), cur);
       last = cur;
@@ -717,15 +664,17 @@ static void sf_gemm_join(const SfGemmArgs &a, hipStream_t st) {
 }
 
 // The launches of one storage type (linear_f32.hip, linear_f16.hip, linear_bf16.hip).
-// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.
-int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
-int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
-int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st);
+// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.  tile 64, 128 or 256, operands as sf_whole_chunks
+// says; layout 0 only: SF_FEW_ROWS, any operands.
+#define SF_FEW_ROWS 16
+int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
+int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
+int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 
-template <typename T, bool PMINOR, bool QMINOR, typename SH, bool DMA>
+template <typename T, bool PMINOR, bool QMINOR, typename SH>
 static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
   static SfSlotCache cache;
-  auto kern = sf_gemm_kernel<T, PMINOR, QMINOR, SH, DMA>;
+  auto kern = sf_gemm_kernel<T, PMINOR, QMINOR, SH>;
   int slots = sf_resident_slots(cache, kern, SH::WAVES * 64, 0, SH::LDS);
   if (slots < 8) {
     sf_set_error("no occupancy for the matrix product kernel on this device");
@@ -740,27 +689,137 @@ static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
 
 typedef SfShape<256, 256, 2, 4, 64, 4, 1> SfTile256;
 typedef SfShape<128, 128, 2, 2, 128, 2, 2> SfTile128;
-typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64;
+// 64 x 64: deep enough to cover the latency of one workgroup alone (64 x 4096 -> 4096 bf16: 33 us with a
+// ring of 2, 21 with 4); fp32's products cover it themselves, three workgroups level the CUs better
+// (35344 x 512 -> 512: 164 us against 168).
+typedef SfShape<64, 64, 2, 2, 128, 4, 2> SfTile64;
+typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64Three;
 
 template <typename T, bool PMINOR, bool QMINOR>
-static int sf_gemm_launch(const SfGemmArgs &a, int tile, bool dma, hipStream_t st) {
+static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
   int rc;
-  if (tile == 256 && dma)
-    rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256, true>(a, st);
-  else if (tile == 128)
-    rc = dma ? sf_gemm_go<T, PMINOR, QMINOR, SfTile128, true>(a, st)
-             : sf_gemm_go<T, PMINOR, QMINOR, SfTile128, false>(a, st);
-  else
-    rc = dma ? sf_gemm_go<T, PMINOR, QMINOR, SfTile64, true>(a, st)
-             : sf_gemm_go<T, PMINOR, QMINOR, SfTile64, false>(a, st);
+  if (tile == 256) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
+  else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
+  else if (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
+  else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
   if (rc) return rc;
   if (a.splits > 1) sf_gemm_join<T>(a, st);
   return SF_OK;
 }
 
+// ---- few rows -------------------------------------------------------------------------------------
+// y of few rows: bound by the weight's bytes and by latency, so there is no tile in LDS
+// and no pipeline.  A workgroup owns 16 columns and 16 TP rows; its 8 waves share the contraction in
+// turns of 64 bytes of k and each loads its operands' fragments straight from memory, all in flight
+// at once (lane = row % 16, 16-byte chunk lane / 16: a row's 64 bytes are one line's half).  The waves'
+// sums meet in LDS and each wave finishes its share of the outputs.
+template <typename T> struct SfMfma16;
+template <> struct SfMfma16<float> {
+  static __device__ __forceinline__ sf_f32x4 run(SfMfma<float>::frag a, SfMfma<float>::frag b, sf_f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+};
+template <> struct SfMfma16<_Float16> {
+  static __device__ __forceinline__ sf_f32x4 run(SfMfma<_Float16>::frag a, SfMfma<_Float16>::frag b,
+                                                 sf_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <> struct SfMfma16<__bf16> {
+  static __device__ __forceinline__ sf_f32x4 run(SfMfma<__bf16>::frag a, SfMfma<__bf16>::frag b,
+                                                 sf_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// Chunk of row `row` (of n) at element i0 (of nk), zeros outside.
 template <typename T>
-static int sf_gemm_any(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st) {
-  if (layout == 0) return sf_gemm_launch<T, false, false>(a, tile, dma, st);
-  if (layout == 1) return sf_gemm_launch<T, false, true>(a, tile, dma, st);
-  return sf_gemm_launch<T, true, true>(a, tile, dma, st);
+__device__ __forceinline__ typename SfMfma<T>::frag sf_row_chunk(const T *p, long long ld, long long row,
+                                                                 long long n, long long i0, long long nk) {
+  constexpr int V = 16 / sizeof(T);
+  typename SfMfma<T>::frag e = {};
+  if (row < n) {
+    const T *at = p + row * ld + i0;
+    if (i0 + V <= nk) {
+      e = __builtin_bit_cast(typename SfMfma<T>::frag, *reinterpret_cast<const sf_u32x4_any *>(at));
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i0 + j < nk) e[j] = at[j];
+    }
+  }
+  return e;
+}
+
+template <typename T, int TP>
+__global__ void __launch_bounds__(512) sf_few_rows_kernel(SfGemmArgs a) {
+  constexpr int V = 16 / sizeof(T), WAVES = 8, UNROLL = 4;
+  __shared__ float part[WAVES][TP][64][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
+  const long long q0 = (long long)(blockIdx.x % a.tiles_q) * 16, p0 = (long long)(blockIdx.x / a.tiles_q) * 16 * TP;
+  const T *p = static_cast<const T *>(a.p), *q = static_cast<const T *>(a.q);
+  sf_f32x4 acc[TP];
+#pragma unroll
+  for (int t = 0; t < TP; ++t) acc[t] = (sf_f32x4){0.f, 0.f, 0.f, 0.f};
+  constexpr int K = 4 * V;      // k of a turn
+  for (long long k0 = wave * K; k0 < a.nk; k0 += UNROLL * WAVES * K) {
+    typename SfMfma<T>::frag fq[UNROLL], fp[UNROLL][TP];
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i) {
+      const long long k = k0 + i * WAVES * K + c * V;
+      fq[i] = sf_row_chunk<T>(q, a.ldq, q0 + r, k < a.nk ? a.nq : 0, k, a.nk);
+#pragma unroll
+      for (int t = 0; t < TP; ++t)
+        fp[i][t] = sf_row_chunk<T>(p, a.ldp, p0 + 16 * t + r, k < a.nk ? a.np : 0, k, a.nk);
+    }
+#pragma unroll
+    for (int i = 0; i < UNROLL; ++i)
+#pragma unroll
+      for (int t = 0; t < TP; ++t) acc[t] = SfMfma16<T>::run(fq[i], fp[i][t], acc[t]);
+  }
+  // accumulator: row p = lane % 16, columns q = 4 (lane / 16) + 0..3
+#pragma unroll
+  for (int t = 0; t < TP; ++t) *reinterpret_cast<sf_f32x4 *>(part[wave][t][lane]) = acc[t];
+  __syncthreads();
+  if (threadIdx.x >= TP * 64) return;
+  const int t = threadIdx.x >> 6;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += part[w][t][lane][j];
+  const long long row = p0 + 16 * t + r, col = q0 + 4 * c;
+  if (row >= a.np) return;
+  const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
+  T *out = static_cast<T *>(a.out), *pre = static_cast<T *>(a.pre);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (col + j >= a.nq) break;
+    const long long at = row * a.nq + col + j;
+    float z = v[j] + (bias ? (float)bias[col + j] : 0.0f);
+    if (pre) pre[at] = (T)z;
+    z = sf_act<T>(z, a.act);
+    out[at] = (T)(z + (res ? (float)res[at] : 0.0f));
+  }
+}
+
+template <typename T>
+static int sf_few_rows(SfGemmArgs a, hipStream_t st) {
+  const int tp = a.np <= 16 ? 1 : a.np <= 32 ? 2 : 4;
+  a.tiles_q = (int)((a.nq + 15) / 16);
+  const dim3 grid((unsigned)(a.tiles_q * ((a.np + 16 * tp - 1) / (16 * tp))));
+  if (tp == 1) hipLaunchKernelGGL((sf_few_rows_kernel<T, 1>), grid, dim3(512), 0, st, a);
+  else if (tp == 2) hipLaunchKernelGGL((sf_few_rows_kernel<T, 2>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((sf_few_rows_kernel<T, 4>), grid, dim3(512), 0, st, a);
+  return SF_OK;
+}
+
+template <typename T>
+static int sf_gemm_any(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
+  if (tile == SF_FEW_ROWS) return sf_few_rows<T>(a, st);
+  if (layout == 0) return sf_gemm_launch<T, false, false>(a, tile, st);
+  if (layout == 1) return sf_gemm_launch<T, false, true>(a, tile, st);
+  return sf_gemm_launch<T, true, true>(a, tile, st);
 }

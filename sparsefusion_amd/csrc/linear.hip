@@ -11,8 +11,9 @@ struct Plan {
   long long k_split;
 };
 
-// Tile and splits of a np x nq product over nk: the cheapest of the three tiles, each with the splits
-// of a long contraction that would fill the chip, by a model of the busiest CU.
+// Tile and splits of a np x nq product over nk: the cheapest of the three tiles, each whole or with the
+// contraction cut into as many parts as fill the chip, by a model of the busiest CU (us; per step of
+// 128 bytes of k, fitted to 20 sizes from 1 x 1024 x 4096 to 8192^3).
 Plan make_plan(long long np, long long nq, long long nk, int dtype) {
   const long long bk = 128 / (long long)sf_dtype_size(dtype);
   const long long steps = (nk + bk - 1) / bk;
@@ -42,13 +43,76 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype) {
 size_t partial_bytes(const Plan &pl, long long np, long long nq) {
   return pl.splits > 1 ? (size_t)pl.splits * np * nq * sizeof(float) : 0;
 }
-size_t align16(size_t v) { return (v + 255) & ~(size_t)255; }
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// Whole aligned chunks along the contiguous axis: the operand can go straight to LDS.  A tile's rows
-// also have to stay in reach of a 31-bit offset.
-bool direct(const void *p, long long ld, long long extent, int dtype) {
-  const long long s = (long long)sf_dtype_size(dtype), v = 16 / s;
-  return (uintptr_t)p % 16 == 0 && ld % v == 0 && extent % v == 0 && ld * s * 256 < 0x7FFFFFFFLL;
+// ---- operands of odd shapes -----------------------------------------------------------------------
+// The tiles load whole aligned 16-byte chunks.  An operand whose rows are not made of such is copied
+// first, rows padded with zeros to whole chunks.  (Loading them through registers was built and timed:
+// 3001 x 451 -> 333 fp16 13.4 us, 32401 x 255 -> 1023 bf16 87 us, both bound by the waits for loads that
+// cannot run ahead.)
+bool whole_chunks(const void *p, long long ld, long long extent, int dtype) {
+  const long long v = 16 / (long long)sf_dtype_size(dtype);
+  return (uintptr_t)p % 16 == 0 && ld % v == 0 && extent % v == 0 && ld <= 2 * SF_LINEAR_MOST_FEATURES;
+}
+long long padded(long long cols, int dtype) {
+  const long long v = 16 / (long long)sf_dtype_size(dtype);
+  return (cols + v - 1) / v * v;
+}
+size_t padded_bytes(long long rows, long long cols, int dtype) {
+  return align256((size_t)rows * padded(cols, dtype) * sf_dtype_size(dtype));
+}
+
+struct Repack {
+  const void *src;
+  void *dst;
+  long long ld, rows, cols;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) repack_kernel(Repack x, Repack y) {
+  constexpr int V = 16 / sizeof(T);
+  const long long cx = (x.cols + V - 1) / V, cy = (y.cols + V - 1) / V;
+  const long long nx = x.rows * cx, n = nx + y.rows * cy;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const Repack &r = i < nx ? x : y;
+    const long long at = i < nx ? i : i - nx, cols = i < nx ? cx : cy, row = at / cols, c = at - row * cols;
+    const T *src = static_cast<const T *>(r.src) + row * r.ld;
+    sf_u32x4 v;
+    if (c * V + V <= r.cols) {
+      v = *reinterpret_cast<const sf_u32x4_any *>(src + c * V);
+    } else {
+      typename SfMfma<T>::frag e;
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = c * V + j < r.cols ? src[c * V + j] : (T)0.0f;
+      v = __builtin_bit_cast(sf_u32x4, e);
+    }
+    static_cast<sf_u32x4 *>(r.dst)[at] = v;
+  }
+}
+
+// Copies x and y (src NULL: not that one) into their padded form.
+int repack(const Repack &x, const Repack &y, int dtype, hipStream_t st) {
+  const long long chunks = (x.src ? x.rows * padded(x.cols, dtype) : 0) +
+                           (y.src ? y.rows * padded(y.cols, dtype) : 0);
+  if (!chunks) return SF_OK;
+  Repack a = x, b = y;
+  if (!a.src) a.rows = a.cols = 0;
+  if (!b.src) b.rows = b.cols = 0;
+  const dim3 grid(sf_grid(chunks / 4, 256));
+  if (dtype == SF_DTYPE_F32) hipLaunchKernelGGL((repack_kernel<float>), grid, dim3(256), 0, st, a, b);
+  else if (dtype == SF_DTYPE_F16) hipLaunchKernelGGL((repack_kernel<_Float16>), grid, dim3(256), 0, st, a, b);
+  else hipLaunchKernelGGL((repack_kernel<__bf16>), grid, dim3(256), 0, st, a, b);
+  SF_CHECK_LAUNCH();
+  return SF_OK;
+}
+
+int launch(const SfGemmArgs &a, int layout, int dtype, int tile, hipStream_t st) {
+  const int rc = dtype == SF_DTYPE_F32   ? sf_gemm_f32(a, layout, tile, st)
+                 : dtype == SF_DTYPE_F16 ? sf_gemm_f16(a, layout, tile, st)
+                                         : sf_gemm_bf16(a, layout, tile, st);
+  if (rc) return rc;
+  SF_CHECK_LAUNCH();
+  return SF_OK;
 }
 
 int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st) {
@@ -62,21 +126,12 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
     SF_CHECK_LAUNCH();
     return SF_OK;
   }
-  const bool dma = direct(a.p, a.ldp, layout == 2 ? a.np : a.nk, dtype) &&
-                   direct(a.q, a.ldq, layout == 0 ? a.nk : a.nq, dtype);
-  const int tile = !dma && pl.tile > 128 ? 128 : pl.tile;      // no 256 tile through registers
-  const long long tp = (a.np + tile - 1) / tile, tq = (a.nq + tile - 1) / tile;
+  const long long tp = (a.np + pl.tile - 1) / pl.tile, tq = (a.nq + pl.tile - 1) / pl.tile;
   SF_CHECK_ARG(tp * tq * pl.splits < SF_INT_MAX, "linear: %lld x %lld outputs are too many for one launch",
                a.np, a.nq);
   a.tiles_p = (int)tp;
   a.tiles_q = (int)tq;
-  int rc;
-  if (dtype == SF_DTYPE_F32) rc = sf_gemm_f32(a, layout, tile, dma, st);
-  else if (dtype == SF_DTYPE_F16) rc = sf_gemm_f16(a, layout, tile, dma, st);
-  else rc = sf_gemm_bf16(a, layout, tile, dma, st);
-  if (rc) return rc;
-  SF_CHECK_LAUNCH();
-  return SF_OK;
+  return launch(a, layout, dtype, pl.tile, st);
 }
 
 // ---- dz and the bias gradient -------------------------------------------------------------------
@@ -85,7 +140,7 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
 // are of the fp32 products, not of the rounded dz.
 template <typename T>
 __global__ void __launch_bounds__(256)
-dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz,
+dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
           float *__restrict__ part, long long m, long long n, long long run) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float red[8][32 * V + 4];
@@ -103,8 +158,10 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
         sf_load_chunk<T>(pre + r * n, col, n, z);
 #pragma unroll
         for (int j = 0; j < V; ++j) g[j] *= sf_act_slope<T>(z[j], act);
-        if (dz) sf_store_chunk<T>(dz + r * n, col, n, g);
       }
+      // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a ReLU's
+      // or GELU's gradient of zero is zero
+      if (dz) sf_store_chunk<T>(dz + r * ldz, col, ldz, g);
 #pragma unroll
       for (int j = 0; j < V; ++j) sum[j] += g[j];
     }
@@ -161,7 +218,7 @@ int run_dz(const void *dy, const void *pre, int act, void *dz, float *part, void
   const int runs = (int)((m + run - 1) / run);
   const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), runs);
   hipLaunchKernelGGL((dz_kernel<T>), grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act,
-                     (T *)dz, db ? part : nullptr, m, n, run);
+                     (T *)dz, padded(n, dtype), db ? part : nullptr, m, n, run);
   SF_CHECK_LAUNCH();
   if (db) {
     hipLaunchKernelGGL((db_join_kernel<T>), dim3(sf_div_up(n, 32)), dim3(1024), 0, st, part, runs, n,
@@ -180,21 +237,51 @@ int zero_out(void *p, long long elements, int dtype, hipStream_t st) {
   return SF_OK;
 }
 
-// Where the pieces of the backward pass's workspace start.
+// Where the pieces of the backward pass's workspace start, and what is copied first.
 struct BackwardPlan {
   Plan dx, dw;
-  size_t dz, part, split, bytes;
+  bool write_dz, pack_x, pack_w;
+  size_t dz, x, w, part, split, bytes;
 };
-BackwardPlan backward_plan(long long m, long long k, long long n, int dtype, int act) {
+BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const void *w, long long m,
+                           long long k, long long n, int dtype, int act) {
   BackwardPlan b;
   b.dx = make_plan(m, k, n, dtype);
   b.dw = make_plan(n, k, m, dtype);
+  b.write_dz = act != SF_ACT_NONE || !whole_chunks(dy, n, n, dtype);
+  b.pack_x = !whole_chunks(x, ldx, k, dtype);
+  b.pack_w = !whole_chunks(w, k, k, dtype);
   b.dz = 0;
-  b.part = act == SF_ACT_NONE ? 0 : align16((size_t)m * n * sf_dtype_size(dtype));
-  b.split = b.part + align16((size_t)dz_runs(m, n, dtype) * n * sizeof(float));
+  b.x = b.write_dz ? padded_bytes(m, n, dtype) : 0;
+  b.w = b.x + (b.pack_x ? padded_bytes(m, k, dtype) : 0);
+  b.part = b.w + (b.pack_w ? padded_bytes(n, k, dtype) : 0);
+  b.split = b.part + align256((size_t)dz_runs(m, n, dtype) * n * sizeof(float));
   const size_t s1 = partial_bytes(b.dx, m, k), s2 = partial_bytes(b.dw, n, k);
   b.bytes = b.split + (s1 > s2 ? s1 : s2);      // the two products run one after the other
   return b;
+}
+
+// The same for the forward pass.
+struct ForwardPlan {
+  Plan y;
+  bool few, pack_x, pack_w;
+  size_t x, w, bytes;
+};
+ForwardPlan forward_plan(const void *x, long long ldx, const void *w, long long m, long long k, long long n,
+                         int dtype) {
+  ForwardPlan f;
+  f.y = make_plan(m, n, k, dtype);
+  f.pack_x = !whole_chunks(x, ldx, k, dtype);
+  f.pack_w = !whole_chunks(w, k, k, dtype);
+  // Few rows go without tiles (16 x 4096 -> 4096 bf16: 10.7 us against 12.1, 1 x 1024 -> 4096: 4.4 against
+  // 8.2, 64 x 4096 -> 4096: 22 against 12.8), more of them where the tiles would need a copy
+  // (64 x 1023 -> 1023 bf16: 21 us).
+  f.few = m <= 16 || (m <= 64 && (f.pack_x || f.pack_w));
+  if (f.few) f.y.splits = 1, f.pack_x = f.pack_w = false;
+  f.x = align256(partial_bytes(f.y, m, n));
+  f.w = f.x + (f.pack_x ? padded_bytes(m, k, dtype) : 0);
+  f.bytes = f.w + (f.pack_w ? padded_bytes(n, k, dtype) : 0);
+  return f;
 }
 
 bool good_sizes(long long m, long long k, long long n, int dtype) {
@@ -210,9 +297,19 @@ bool good_sizes(long long m, long long k, long long n, int dtype) {
 
 }  // namespace
 
-extern "C" size_t sf_linear_workspace(long long m, long long k, long long n, int dtype) {
-  if (!good_sizes(m, k, n, dtype) || !m || !n) return 0;
-  return partial_bytes(make_plan(m, n, k, dtype), m, n);
+#define SF_LINEAR_CHECK_WORKSPACE(name, need)                                                      \
+  do {                                                                                             \
+    if ((need) && (!ws || ws_bytes < (need))) {                                                    \
+      sf_set_error("%s needs %zu bytes of workspace, got %zu", name, (size_t)(need), ws_bytes);    \
+      return SF_ERR_WORKSPACE;                                                                     \
+    }                                                                                              \
+    SF_CHECK_ARG(!(need) || (uintptr_t)ws % 16 == 0, "%s: workspace is not 16-byte aligned", name); \
+  } while (0)
+
+extern "C" size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
+                                      long long k, long long n, int dtype) {
+  if (!good_sizes(m, k, n, dtype) || !m || !n || !k) return 0;
+  return forward_plan(x, ldx, weight, m, k, n, dtype).bytes;
 }
 
 extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const void *bias,
@@ -221,25 +318,32 @@ extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const
   SF_LINEAR_CHECK();
   if (m == 0 || n == 0) return SF_OK;
   SF_CHECK_ARG(y && ((x && weight) || k == 0), "NULL tensor pointer");
-  const Plan pl = make_plan(m, n, k, dtype);
-  const size_t need = partial_bytes(pl, m, n);
-  if (need && (!ws || ws_bytes < need)) {
-    sf_set_error("sf_linear needs %zu bytes of workspace, got %zu", need, ws_bytes);
-    return SF_ERR_WORKSPACE;
-  }
+  const hipStream_t st = (hipStream_t)stream;
   SfGemmArgs a{};
   a.p = x, a.q = weight, a.ldp = ldx, a.ldq = k;
   a.np = m, a.nq = n, a.nk = k;
   a.bias = bias, a.residual = residual, a.out = y, a.pre = pre;
-  a.partial = (float *)ws;
   a.act = act;
-  return product(a, 0, dtype, pl, (hipStream_t)stream);
+  if (k == 0) return product(a, 0, dtype, make_plan(m, n, k, dtype), st);
+  const ForwardPlan f = forward_plan(x, ldx, weight, m, k, n, dtype);
+  if (f.few) return launch(a, 0, dtype, SF_FEW_ROWS, st);
+  SF_LINEAR_CHECK_WORKSPACE("sf_linear", f.bytes);
+  unsigned char *base = (unsigned char *)ws;
+  a.partial = (float *)base;
+  const Repack px{f.pack_x ? x : nullptr, base + f.x, ldx, m, k};
+  const Repack pw{f.pack_w ? weight : nullptr, base + f.w, k, n, k};
+  const int rc = repack(px, pw, dtype, st);
+  if (rc) return rc;
+  if (f.pack_x) a.p = px.dst, a.ldp = padded(k, dtype);
+  if (f.pack_w) a.q = pw.dst, a.ldq = padded(k, dtype);
+  return product(a, 0, dtype, f.y, st);
 }
 
-extern "C" size_t sf_linear_backward_workspace(long long m, long long k, long long n, int dtype,
-                                               int act) {
+extern "C" size_t sf_linear_backward_workspace(const void *dy, const void *x, long long ldx,
+                                               const void *weight, long long m, long long k,
+                                               long long n, int dtype, int act) {
   if (!good_sizes(m, k, n, dtype) || !m || !n) return 0;
-  return backward_plan(m, k, n, dtype, act).bytes;
+  return backward_plan(dy, x, ldx, weight, m, k, n, dtype, act).bytes;
 }
 
 extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, const void *weight,
@@ -253,29 +357,29 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
     if ((rc = zero_out(dx, m * k, dtype, st)) || (rc = zero_out(dw, n * k, dtype, st))) return rc;
     return zero_out(db, n, dtype, st);
   }
-  SF_CHECK_ARG(dy && (pre || act == SF_ACT_NONE) && (weight || !dx || !k) && (x || !dw || !k),
-               "NULL tensor pointer");
-  const BackwardPlan b = backward_plan(m, k, n, dtype, act);
-  if (b.bytes && (!ws || ws_bytes < b.bytes)) {
-    sf_set_error("sf_linear_backward needs %zu bytes of workspace, got %zu", b.bytes, ws_bytes);
-    return SF_ERR_WORKSPACE;
-  }
+  if (k == 0) dx = dw = nullptr;
+  SF_CHECK_ARG(dy && (pre || act == SF_ACT_NONE) && (weight || !dx) && (x || !dw), "NULL tensor pointer");
+  const BackwardPlan b = backward_plan(dy, x, ldx, weight, m, k, n, dtype, act);
+  SF_LINEAR_CHECK_WORKSPACE("sf_linear_backward", b.bytes);
   unsigned char *base = (unsigned char *)ws;
   const void *dz = dy;
-  const bool products = (dx || dw) && k > 0;
-  if (db || (act != SF_ACT_NONE && products)) {
-    void *out = act != SF_ACT_NONE && products ? base + b.dz : nullptr;
+  long long ldz = n;
+  const bool write_dz = b.write_dz && (dx || dw);
+  if (db || write_dz) {
+    void *out = write_dz ? base + b.dz : nullptr;
     float *part = (float *)(base + b.part);
     if (dtype == SF_DTYPE_F32) rc = run_dz<float>(dy, pre, act, out, part, db, m, n, dtype, st);
     else if (dtype == SF_DTYPE_F16) rc = run_dz<_Float16>(dy, pre, act, out, part, db, m, n, dtype, st);
     else rc = run_dz<__bf16>(dy, pre, act, out, part, db, m, n, dtype, st);
     if (rc) return rc;
-    if (out) dz = out;
+    if (out) dz = out, ldz = padded(n, dtype);
   }
-  if (k == 0) return SF_OK;
+  const Repack px{b.pack_x && dw ? x : nullptr, base + b.x, ldx, m, k};
+  const Repack pw{b.pack_w && dx ? weight : nullptr, base + b.w, k, n, k};
+  if ((rc = repack(px, pw, dtype, st))) return rc;
   if (dx) {
     SfGemmArgs a{};
-    a.p = dz, a.q = weight, a.ldp = n, a.ldq = k;
+    a.p = dz, a.q = pw.src ? pw.dst : weight, a.ldp = ldz, a.ldq = pw.src ? padded(k, dtype) : k;
     a.np = m, a.nq = k, a.nk = n;
     a.out = dx;
     a.partial = (float *)(base + b.split);
@@ -283,7 +387,7 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   }
   if (dw) {
     SfGemmArgs a{};
-    a.p = dz, a.q = x, a.ldp = n, a.ldq = ldx;
+    a.p = dz, a.q = px.src ? px.dst : x, a.ldp = ldz, a.ldq = px.src ? padded(k, dtype) : ldx;
     a.np = n, a.nq = k, a.nk = m;
     a.out = dw;
     a.partial = (float *)(base + b.split);

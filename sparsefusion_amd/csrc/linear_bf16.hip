@@ -2,6 +2,6 @@
 // storage type so that the kernels compile side by side.
 #include "gemm_tile.h"
 
-int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, bool dma, hipStream_t st) {
-  return sf_gemm_any<__bf16>(a, layout, tile, dma, st);
+int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
+  return sf_gemm_any<__bf16>(a, layout, tile, st);
 }

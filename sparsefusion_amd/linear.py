@@ -67,10 +67,11 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     y = x.new_empty(shape)
     pre = x.new_empty(shape) if keep_pre else None
     L = _lib.lib()
-    nbytes = L.sf_linear_workspace(m, k, n, code)
+    px, pw = rows.data_ptr(), weight.data_ptr()
+    nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code)
     ws = _lib.workspace(nbytes, x)
     rc = L.sf_linear(
-        rows.data_ptr(), ldx, weight.data_ptr(), None if bias is None else bias.data_ptr(),
+        px, ldx, pw, None if bias is None else bias.data_ptr(),
         None if residual is None else residual.data_ptr(), y.data_ptr(),
         None if pre is None else pre.data_ptr(), m, k, n, code, act,
         None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
@@ -107,10 +108,11 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     dw = x.new_empty((n, k)) if needs[1] else None
     db = x.new_empty(n) if needs[2] else None
     L = _lib.lib()
-    nbytes = L.sf_linear_backward_workspace(m, k, n, code, act)
+    pg, px, pw = grad.data_ptr(), rows.data_ptr(), weight.data_ptr()
+    nbytes = L.sf_linear_backward_workspace(pg, px, ldx, pw, m, k, n, code, act)
     ws = _lib.workspace(nbytes, x)
     rc = L.sf_linear_backward(
-        grad.data_ptr(), rows.data_ptr(), ldx, weight.data_ptr(),
+        pg, px, ldx, pw,
         None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
         None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code,
         act, None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
