@@ -9,12 +9,14 @@ import subprocess
 
 import torch
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream wraps
+_get_device = torch._C._cuda_getDevice
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libsparsefusion_hip.so')
 _LIB = None
 
 SF_OK = 0
+SF_ERR_WORKSPACE = -2
 
 _vp, _i, _sz, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_longlong
 _F3, _F6, _I3 = C.c_float * 3, C.c_float * 6, C.c_int * 3   # array instances decay to pointers
@@ -192,7 +194,7 @@ def elsewhere(device):
     if device.type != 'cuda':
         raise RuntimeError('sparsefusion_amd ops need tensors on a HIP device '
                            f'(got {device}); there is no CPU path')
-    return device.index != torch.cuda.current_device()
+    return device.index != _get_device()
 
 
 def same(x, name, t):
@@ -218,15 +220,6 @@ def workspace(nbytes, x):
     current stream's pool when the caller drops it and is handed out again in that stream's order only;
     under capture it belongs to the graph's own pool."""
     return x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-
-
-def differentiable(*tensors):
-    """Whether autograd would record an operation on these tensors."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
 
 
 class _ForwardOnly(torch.autograd.Function):

@@ -479,8 +479,9 @@ __device__ __forceinline__ void sf_wait_loads() {
   __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0070);
 }
 
+// Workgroup `group` of `groups`, which share the tiles of the product.
 template <typename T, bool PMINOR, bool QMINOR, typename SH>
-__global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_gemm_kernel(SfGemmArgs a) {
+__device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds, int group, int groups) {
   constexpr int BP = SH::BP, BQ = SH::BQ, WQ = SH::WQ, WAVES = SH::WAVES, STEP = SH::STEP;
   constexpr int RING = SH::RING, BYTES = SH::BYTES, BK = STEP / (int)sizeof(T), NS = STEP / 32;
   constexpr int TP = BP / SH::WP / 32, TQ = BQ / WQ / 32;
@@ -488,7 +489,6 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
   typedef SfOperand<T, QMINOR, BQ, WAVES, STEP> OQ;
   typedef typename SfMfma<T>::frag frag;
   constexpr int NI = OP::NI + OQ::NI;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wp = wave / WQ, wq = wave % WQ;
   float *stage = reinterpret_cast<float *>(lds + RING * BYTES) + wave * 1024;
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
   OQ oq;
   op.init(a.ldp, wave, lane);
   oq.init(a.ldq, wave, lane);
-  int lt = blockIdx.x;
+  int lt = group;
   auto open = [&]() {
     int tp, tq, split;
     sf_tile_of(lt, tiles, a, &tp, &tq, &split);
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
   auto advance = [&]() {      // behind the last instruction of a step's load
     op.next(), oq.next();
     if (op.steps == 0) {
-      lt += gridDim.x;
+      lt += groups;
       if (lt < tiles) open();
       else op.close(), oq.close();
     }
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
   sf_wait_loads<(RING - 2) * NI + HALF>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+  for (int tile = group; tile < tiles; tile += groups) {
     int tp, tq, split;
     sf_tile_of(tile, tiles, a, &tp, &tq, &split);
     const int steps = sf_steps<BK>(a, split);
@@ -622,6 +622,12 @@ __global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_ge
   sf_wait_loads<0>();      // the loads of nothing still write zeros into this workgroup's LDS
 }
 
+template <typename T, bool PMINOR, bool QMINOR, typename SH>
+__global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4) sf_gemm_kernel(SfGemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
+  sf_gemm<T, PMINOR, QMINOR, SH>(a, lds, blockIdx.x, gridDim.x);
+}
+
 // Adds the splits' partial sums in order and applies the epilogue; rows of one chunk a lane.
 template <typename T>
 __global__ void __launch_bounds__(256) sf_gemm_join_kernel(SfGemmArgs a) {
@@ -670,6 +676,11 @@ static void sf_gemm_join(const SfGemmArgs &a, hipStream_t st) {
 int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
+// Both gradients' products, 64 x 64 tiles without splits, and the bias gradient's sum.
+struct SfColumnSums;
+int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
+int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
+int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 
 template <typename T, bool PMINOR, bool QMINOR, typename SH>
 static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
@@ -704,6 +715,54 @@ static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
   else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
   if (rc) return rc;
   if (a.splits > 1) sf_gemm_join<T>(a, st);
+  return SF_OK;
+}
+
+// ---- a small layer's gradients in one launch --------------------------------------------------------
+// Sums of `runs` partial rows of n, 32 columns by 8 strided runs of rows a workgroup of 256.
+struct SfColumnSums {
+  const float *part;      // (runs, n)
+  void *out;              // (n) of T, or NULL: nothing to do
+  long long n;
+  int runs;
+};
+template <typename T>
+__device__ __forceinline__ void sf_join_columns(const SfColumnSums &c, int group, float *red) {
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const long long i = (long long)group * 32 + tx;
+  float t = 0.0f;
+  if (i < c.n) {
+#pragma unroll 8
+    for (int b = ty; b < c.runs; b += 8) t += c.part[b * c.n + i];
+  }
+  red[ty * 33 + tx] = t;
+  __syncthreads();
+  if (ty == 0 && i < c.n) {
+    float v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += red[k * 33 + tx];
+    static_cast<T *>(c.out)[i] = (T)v;
+  }
+}
+
+// dx = dz w, dw = dz^T x and db's last sum by different workgroups of one launch: products of a few tiles
+// each are all latency (400 x 256 -> 128 fp32: 7 us each, one behind the other, and a launch more).
+template <typename T, typename SH>
+__global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4)
+sf_gradients_kernel(SfGemmArgs dx, int dx_groups, SfGemmArgs dw, int dw_groups, SfColumnSums db) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
+  const int g = blockIdx.x;
+  if (g < dx_groups) sf_gemm<T, false, true, SH>(dx, lds, g, dx_groups);
+  else if (g < dx_groups + dw_groups) sf_gemm<T, true, true, SH>(dw, lds, g - dx_groups, dw_groups);
+  else sf_join_columns<T>(db, g - dx_groups - dw_groups, reinterpret_cast<float *>(lds));
+}
+
+template <typename T>
+static int sf_gradients_go(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
+  const int nx = dx.tiles_p * dx.tiles_q, nw = dw.tiles_p * dw.tiles_q;
+  const int nb = db.out ? (int)((db.n + 31) / 32) : 0;
+  hipLaunchKernelGGL((sf_gradients_kernel<T, SfTile64Three>), dim3(nx + nw + nb), dim3(256), 0, st, dx, nx, dw,
+                     nw, db);
   return SF_OK;
 }
 

@@ -24,16 +24,19 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype) {
     const long long t = ((np + tile - 1) / tile) * ((nq + tile - 1) / tile);
     for (int full = 0; full < 2; ++full) {
       const int slots = 256 * (tile == 256 ? 1 : tile == 128 ? 2 : 3);
-      long long s = full ? slots / t : 1;
-      if (s > steps / 4) s = steps / 4;
-      if (s < 1 || (full && s == 1)) continue;
+      long long s = 1;
+      if (full) {
+        s = slots / t < steps / 4 ? slots / t : steps / 4;
+        if (s < 2) continue;
+      }
       const long long per = (steps + s - 1) / s;
       s = (steps + per - 1) / per;
-      const double n = (double)((t * s + 255) / 256);
+      const long long n = (t * s + 255) / 256;      // workgroups of the busiest CU, one after the other but:
+      const double pairs = (double)((n + 1) / 2);   // two 128 tiles take hardly longer than one
       double c = dtype == SF_DTYPE_F32
-                     ? n * (tile == 256 ? 8 + 7.9 * per : tile == 128 ? 2 + 2.05 * per : 0.7 + 0.55 * per)
-                     : n * (tile == 256 ? 8 + 1.5 * per : tile == 128 ? 2 + 0.48 * per : 0.8 + 0.21 * per);
-      if (s > 1) c += 3 + 8e-6 * (double)(np * nq * s) / 4.5;
+                     ? n * (tile == 256 ? 8 + 7.5 * per : tile == 128 ? 2 + 2.05 * per : 0.7 + 0.57 * per)
+                     : tile == 256 ? n * (8 + 1.75 * per) : tile == 128 ? pairs * (4 + per) : n * (0.8 + 0.3 * per);
+      if (s > 1) c += 6 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
       if (c < least) least = c, best = Plan{tile, (int)s, per * bk};
     }
   }
@@ -115,9 +118,16 @@ int launch(const SfGemmArgs &a, int layout, int dtype, int tile, hipStream_t st)
   return SF_OK;
 }
 
-int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st) {
+// The plan into the arguments; false if it has too many tiles.
+bool prepare(SfGemmArgs &a, const Plan &pl) {
+  const long long tp = (a.np + pl.tile - 1) / pl.tile, tq = (a.nq + pl.tile - 1) / pl.tile;
+  a.tiles_p = (int)tp, a.tiles_q = (int)tq;
   a.splits = pl.splits;
   a.k_split = pl.k_split;
+  return tp * tq * pl.splits < SF_INT_MAX;
+}
+
+int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st) {
   if (a.nk == 0) {      // nothing to sum: the epilogue alone
     a.splits = 0;
     if (dtype == SF_DTYPE_F32) sf_gemm_join<float>(a, st);
@@ -126,11 +136,7 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
     SF_CHECK_LAUNCH();
     return SF_OK;
   }
-  const long long tp = (a.np + pl.tile - 1) / pl.tile, tq = (a.nq + pl.tile - 1) / pl.tile;
-  SF_CHECK_ARG(tp * tq * pl.splits < SF_INT_MAX, "linear: %lld x %lld outputs are too many for one launch",
-               a.np, a.nq);
-  a.tiles_p = (int)tp;
-  a.tiles_q = (int)tq;
+  SF_CHECK_ARG(prepare(a, pl), "linear: %lld x %lld outputs are too many for one launch", a.np, a.nq);
   return launch(a, layout, dtype, pl.tile, st);
 }
 
@@ -142,7 +148,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
           float *__restrict__ part, long long m, long long n, long long run) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), DEEP = 4;
   __shared__ float red[8][32 * V + 4];
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const long long col = ((long long)blockIdx.x * 32 + cl) * V;
@@ -151,19 +157,28 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.0f;
   if (col < n)
-    for (long long r = r0 + rl; r < r1; r += 8) {
-      float g[V], z[V];
-      sf_load_chunk<T>(dy + r * n, col, n, g);
-      if (act != SF_ACT_NONE) {
-        sf_load_chunk<T>(pre + r * n, col, n, z);
+    for (long long r = r0 + rl; r < r1; r += 8 * DEEP) {
+      // DEEP rows' loads in flight; rows past the run are read again and count for nothing
+      float g[DEEP][V], z[DEEP][V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) g[j] *= sf_act_slope<T>(z[j], act);
+      for (int i = 0; i < DEEP; ++i) {
+        const long long row = r + 8 * i < r1 ? r + 8 * i : r;
+        sf_load_chunk<T>(dy + row * n, col, n, g[i]);
+        if (act != SF_ACT_NONE) sf_load_chunk<T>(pre + row * n, col, n, z[i]);
       }
-      // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a ReLU's
-      // or GELU's gradient of zero is zero
-      if (dz) sf_store_chunk<T>(dz + r * ldz, col, ldz, g);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += g[j];
+      for (int i = 0; i < DEEP; ++i) {
+        if (r + 8 * i >= r1) break;
+        if (act != SF_ACT_NONE) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[i][j] *= sf_act_slope<T>(z[i][j], act);
+        }
+        // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a
+        // ReLU's or GELU's gradient of zero is zero
+        if (dz) sf_store_chunk<T>(dz + (r + 8 * i) * ldz, col, ldz, g[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += g[i][j];
+      }
     }
   if (!part) return;
 #pragma unroll
@@ -180,24 +195,9 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
 }
 
 template <typename T>
-__global__ void __launch_bounds__(1024)
-db_join_kernel(const float *__restrict__ part, int runs, long long n, T *__restrict__ db) {
-  __shared__ float red[32][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const long long i = (long long)blockIdx.x * 32 + tx;
-  float t = 0.0f;
-  if (i < n) {
-#pragma unroll 8
-    for (int b = ty; b < runs; b += 32) t += part[b * n + i];
-  }
-  red[ty][tx] = t;
-  __syncthreads();
-  if (ty == 0 && i < n) {
-    float a = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) a += red[k][tx];
-    db[i] = (T)a;
-  }
+__global__ void __launch_bounds__(256) db_join_kernel(SfColumnSums c) {
+  __shared__ float red[8 * 33];
+  sf_join_columns<T>(c, blockIdx.x, red);
 }
 
 // Runs of rows of dz_kernel: about 2048 workgroups in all, at least 32 rows each.
@@ -209,23 +209,23 @@ int dz_runs(long long m, long long n, int dtype) {
   return (int)(runs < 1 ? 1 : runs);
 }
 
+// dz (or NULL) and the partial sums for db (or NULL).
 template <typename T>
-int run_dz(const void *dy, const void *pre, int act, void *dz, float *part, void *db, long long m,
-           long long n, int dtype, hipStream_t st) {
+void run_dz(const void *dy, const void *pre, int act, void *dz, SfColumnSums &db, float *part, long long m,
+            long long n, int dtype, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const int want = dz_runs(m, n, dtype);
   const long long run = (m + want - 1) / want;
-  const int runs = (int)((m + run - 1) / run);
-  const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), runs);
-  hipLaunchKernelGGL((dz_kernel<T>), grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act,
-                     (T *)dz, padded(n, dtype), db ? part : nullptr, m, n, run);
-  SF_CHECK_LAUNCH();
-  if (db) {
-    hipLaunchKernelGGL((db_join_kernel<T>), dim3(sf_div_up(n, 32)), dim3(1024), 0, st, part, runs, n,
-                       (T *)db);
-    SF_CHECK_LAUNCH();
-  }
-  return SF_OK;
+  db.part = part, db.n = n, db.runs = (int)((m + run - 1) / run);
+  const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), db.runs);
+  hipLaunchKernelGGL((dz_kernel<T>), grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act, (T *)dz,
+                     padded(n, dtype), db.out ? part : nullptr, m, n, run);
+}
+void join_db(const SfColumnSums &db, int dtype, hipStream_t st) {
+  const dim3 grid(sf_div_up(db.n, 32));
+  if (dtype == SF_DTYPE_F32) hipLaunchKernelGGL((db_join_kernel<float>), grid, dim3(256), 0, st, db);
+  else if (dtype == SF_DTYPE_F16) hipLaunchKernelGGL((db_join_kernel<_Float16>), grid, dim3(256), 0, st, db);
+  else hipLaunchKernelGGL((db_join_kernel<__bf16>), grid, dim3(256), 0, st, db);
 }
 
 int zero_out(void *p, long long elements, int dtype, hipStream_t st) {
@@ -365,33 +365,44 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   const void *dz = dy;
   long long ldz = n;
   const bool write_dz = b.write_dz && (dx || dw);
+  SfColumnSums sums{};
+  sums.out = db;
   if (db || write_dz) {
     void *out = write_dz ? base + b.dz : nullptr;
     float *part = (float *)(base + b.part);
-    if (dtype == SF_DTYPE_F32) rc = run_dz<float>(dy, pre, act, out, part, db, m, n, dtype, st);
-    else if (dtype == SF_DTYPE_F16) rc = run_dz<_Float16>(dy, pre, act, out, part, db, m, n, dtype, st);
-    else rc = run_dz<__bf16>(dy, pre, act, out, part, db, m, n, dtype, st);
-    if (rc) return rc;
+    if (dtype == SF_DTYPE_F32) run_dz<float>(dy, pre, act, out, sums, part, m, n, dtype, st);
+    else if (dtype == SF_DTYPE_F16) run_dz<_Float16>(dy, pre, act, out, sums, part, m, n, dtype, st);
+    else run_dz<__bf16>(dy, pre, act, out, sums, part, m, n, dtype, st);
+    SF_CHECK_LAUNCH();
     if (out) dz = out, ldz = padded(n, dtype);
   }
   const Repack px{b.pack_x && dw ? x : nullptr, base + b.x, ldx, m, k};
   const Repack pw{b.pack_w && dx ? weight : nullptr, base + b.w, k, n, k};
   if ((rc = repack(px, pw, dtype, st))) return rc;
-  if (dx) {
-    SfGemmArgs a{};
-    a.p = dz, a.q = pw.src ? pw.dst : weight, a.ldp = ldz, a.ldq = pw.src ? padded(k, dtype) : k;
-    a.np = m, a.nq = k, a.nk = n;
-    a.out = dx;
-    a.partial = (float *)(base + b.split);
-    if ((rc = product(a, 1, dtype, b.dx, st))) return rc;
+  SfGemmArgs gx{}, gw{};
+  gx.p = dz, gx.q = pw.src ? pw.dst : weight, gx.ldp = ldz, gx.ldq = pw.src ? padded(k, dtype) : k;
+  gx.np = m, gx.nq = k, gx.nk = n;
+  gx.out = dx;
+  gw.p = dz, gw.q = px.src ? px.dst : x, gw.ldp = ldz, gw.ldq = px.src ? padded(k, dtype) : ldx;
+  gw.np = n, gw.nq = k, gw.nk = m;
+  gw.out = dw;
+  gx.partial = gw.partial = (float *)(base + b.split);
+  // one launch while every workgroup of both products is resident at once
+  if (dx && dw && b.dx.tile == 64 && b.dw.tile == 64 && b.dx.splits == 1 && b.dw.splits == 1 &&
+      prepare(gx, b.dx) && prepare(gw, b.dw) &&
+      (long long)gx.tiles_p * gx.tiles_q + (long long)gw.tiles_p * gw.tiles_q <= 768) {
+    rc = dtype == SF_DTYPE_F32   ? sf_gradients_f32(gx, gw, sums, st)
+         : dtype == SF_DTYPE_F16 ? sf_gradients_f16(gx, gw, sums, st)
+                                 : sf_gradients_bf16(gx, gw, sums, st);
+    if (rc) return rc;
+    SF_CHECK_LAUNCH();
+    return SF_OK;
   }
-  if (dw) {
-    SfGemmArgs a{};
-    a.p = dz, a.q = px.src ? px.dst : x, a.ldp = ldz, a.ldq = px.src ? padded(k, dtype) : ldx;
-    a.np = n, a.nq = k, a.nk = m;
-    a.out = dw;
-    a.partial = (float *)(base + b.split);
-    if ((rc = product(a, 2, dtype, b.dw, st))) return rc;
+  if (db) {
+    join_db(sums, dtype, st);
+    SF_CHECK_LAUNCH();
   }
+  if (dx && (rc = product(gx, 1, dtype, b.dx, st))) return rc;
+  if (dw && (rc = product(gw, 2, dtype, b.dw, st))) return rc;
   return SF_OK;
 }

@@ -5,3 +5,6 @@
 int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
   return sf_gemm_any<__bf16>(a, layout, tile, st);
 }
+int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
+  return sf_gradients_go<__bf16>(dx, dw, db, st);
+}

@@ -5,3 +5,6 @@
 int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
   return sf_gemm_any<_Float16>(a, layout, tile, st);
 }
+int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
+  return sf_gradients_go<_Float16>(dx, dw, db, st);
+}

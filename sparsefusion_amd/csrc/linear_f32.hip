@@ -5,3 +5,6 @@
 int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
   return sf_gemm_any<float>(a, layout, tile, st);
 }
+int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
+  return sf_gradients_go<float>(dx, dw, db, st);
+}

@@ -154,7 +154,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=Fa
     """Layer norm of x + residual over the last dimension, differentiable in all four tensors; with
     return_sum -> (y, sum), for blocks that carry the sum on.  weight and bias (D,) or None; residual
     has x's shape or expands to it (its gradient is summed back)."""
-    if _lib.differentiable(x, weight, bias, residual):
+    if (x.requires_grad or (weight is not None and weight.requires_grad) or
+            (bias is not None and bias.requires_grad) or
+            (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         if residual is not None and residual.shape != x.shape:
             residual = residual.expand(x.shape)
         return _LayerNorm.apply(x, weight, bias, eps, residual, return_sum)

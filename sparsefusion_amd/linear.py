@@ -37,7 +37,8 @@ def _check(x, weight):
         raise RuntimeError(f'expected rows of {k} elements, got {tuple(x.shape)}')
     if max(n, k) > MOST_FEATURES:
         raise RuntimeError(f'linear takes up to {MOST_FEATURES} features, got {k} -> {n}')
-    _lib.same(x, 'weight', weight)
+    if weight.dtype != x.dtype or weight.device != x.device:
+        _lib.same(x, 'weight', weight)
     return n, k, code
 
 
@@ -49,7 +50,8 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     n, k, code = _check(x, weight)
     shape = (x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n)
     if bias is not None:
-        _lib.same(x, 'bias', bias)
+        if bias.dtype != x.dtype or bias.device != x.device:
+            _lib.same(x, 'bias', bias)
         if bias.dim() != 1 or bias.shape[0] != n:
             raise RuntimeError(f'bias must have shape ({n},), got {tuple(bias.shape)}')
         bias = bias.contiguous()
@@ -68,13 +70,15 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     pre = x.new_empty(shape) if keep_pre else None
     L = _lib.lib()
     px, pw = rows.data_ptr(), weight.data_ptr()
-    nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code)
-    ws = _lib.workspace(nbytes, x)
-    rc = L.sf_linear(
-        px, ldx, pw, None if bias is None else bias.data_ptr(),
-        None if residual is None else residual.data_ptr(), y.data_ptr(),
-        None if pre is None else pre.data_ptr(), m, k, n, code, act,
-        None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
+    args = (px, ldx, pw, None if bias is None else bias.data_ptr(),
+            None if residual is None else residual.data_ptr(), y.data_ptr(),
+            None if pre is None else pre.data_ptr(), m, k, n, code, act)
+    # most sizes need no scratch: only a refusal asks how much
+    rc = L.sf_linear(*args, None, 0, _lib.stream(x.device))
+    if rc == _lib.SF_ERR_WORKSPACE:
+        nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        rc = L.sf_linear(*args, ws.data_ptr(), nbytes, _lib.stream(x.device))
     if rc:
         _lib.check(rc)
     return y, pre
@@ -148,7 +152,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x @ weight.T + bias) + residual, differentiable in all four tensors.  x (..., K), weight
     (N, K), bias (N,); activation None, 'relu' or 'gelu'; residual (..., N) or anything that expands
     to it (its gradient is summed back)."""
-    if _lib.differentiable(x, weight, bias, residual):
+    if (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+            (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         if residual is not None and x.dim() and residual.shape != x.shape[:-1] + weight.shape[:1]:
             residual = residual.expand(x.shape[:-1] + weight.shape[:1])
         return _Linear.apply(x, weight, bias, activation, residual)
