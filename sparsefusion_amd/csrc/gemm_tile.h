@@ -732,8 +732,13 @@ __device__ __forceinline__ void sf_join_columns(const SfColumnSums &c, int group
   const long long i = (long long)group * 32 + tx;
   float t = 0.0f;
   if (i < c.n) {
-#pragma unroll 8
-    for (int b = ty; b < c.runs; b += 8) t += c.part[b * c.n + i];
+    for (int b0 = ty; b0 < c.runs; b0 += 16 * 8) {      // 16 loads in flight
+      float u[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) u[k] = b0 + 8 * k < c.runs ? c.part[(b0 + 8 * k) * c.n + i] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) t += u[k];
+    }
   }
   red[ty * 33 + tx] = t;
   __syncthreads();

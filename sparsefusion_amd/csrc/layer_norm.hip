@@ -50,7 +50,7 @@ __device__ __forceinline__ void load_param(const void *p, int i0, int n, float f
   for (int j = 0; j < V; ++j) v[j] = (q && i0 + j < n) ? (float)q[i0 + j] : fallback;
 }
 
-template <typename T, typename P, int LANES, int NV, int THREADS>
+template <typename T, typename P, int LANES, int NV, int THREADS, bool NT>
 __global__ void __launch_bounds__(THREADS)
 norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *w, const void *b,
                 T *__restrict__ y, T *__restrict__ sum, float *__restrict__ mean,
@@ -74,10 +74,10 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int i0 = (c * LANES + lane) * V;
-      sf_load_chunk<T>(x + at, i0, d, v[c]);
+      sf_load_chunk<T, NT>(x + at, i0, d, v[c]);
       if (res) {
         float u[V];
-        sf_load_chunk<T>(res + at, i0, d, u);
+        sf_load_chunk<T, NT>(res + at, i0, d, u);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[c][j] += u[j];
       }
@@ -161,7 +161,7 @@ norm_fwd_long_kernel(const T *__restrict__ x, const T *__restrict__ res, const v
 }
 
 // dx of every row and, in part[block][2][d] (fp32), the workgroup's share of dw and db.
-template <typename T, typename P, int LANES, int NV, int THREADS>
+template <typename T, typename P, int LANES, int NV, int THREADS, bool NT>
 __global__ void __launch_bounds__(THREADS)
 norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *w, const T *__restrict__ dsum,
@@ -188,8 +188,8 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int i0 = (c * LANES + lane) * V;
-      sf_load_chunk<T>(dy + at, i0, d, g[c]);
-      sf_load_chunk<T>(x + at, i0, d, xh[c]);
+      sf_load_chunk<T, NT>(dy + at, i0, d, g[c]);
+      sf_load_chunk<T, NT>(x + at, i0, d, xh[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         // g is zero behind the row's end, so xh there (a product of nothing but the mean) is harmless
@@ -212,7 +212,7 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
       const int i0 = (c * LANES + lane) * V;
       float u[V];
       if (dsum) {
-        sf_load_chunk<T>(dsum + at, i0, d, u);
+        sf_load_chunk<T, NT>(dsum + at, i0, d, u);
       } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] = 0.0f;
@@ -325,8 +325,14 @@ norm_join_kernel(const float *__restrict__ part, int blocks, int d, P *__restric
   const int i = blockIdx.x * 32 + tx;      // of the 2 d sums
   float t = 0.0f;
   if (i < 2 * d) {
-#pragma unroll 8
-    for (int b = ty; b < blocks; b += 32) t += part[(size_t)b * 2 * d + i];
+    // 16 loads in flight: this kernel is nothing but their latency
+    for (int b0 = ty; b0 < blocks; b0 += 16 * 32) {
+      float u[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) u[k] = b0 + 32 * k < blocks ? part[(size_t)(b0 + 32 * k) * 2 * d + i] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) t += u[k];
+    }
   }
   red[ty][tx] = t;
   __syncthreads();
@@ -385,15 +391,17 @@ int bwd_blocks(long long m, int d, int dtype) {
 }
 
 #define SF_NORM_SHAPES(GO)                                                             \
-  if (s.lanes == 8) GO(8, 1, 256);                                                     \
-  else if (s.lanes == 16) GO(16, 1, 256);                                              \
-  else if (s.lanes == 32) GO(32, 1, 256);                                              \
-  else if (s.lanes == 64 && s.nv == 1) GO(64, 1, 256);                                 \
-  else if (s.lanes == 64) GO(64, 2, 256);                                              \
-  else if (s.lanes == 256 && s.nv == 1) GO(256, 1, 256);                               \
-  else if (s.lanes == 256) GO(256, 2, 256);                                            \
-  else if (s.nv == 1) GO(1024, 1, 1024);                                               \
-  else GO(1024, 2, 1024)
+  do {                                                                                 \
+    if (s.lanes == 8) { GO(8, 1, 256); }                                               \
+    else if (s.lanes == 16) { GO(16, 1, 256); }                                        \
+    else if (s.lanes == 32) { GO(32, 1, 256); }                                        \
+    else if (s.lanes == 64 && s.nv == 1) { GO(64, 1, 256); }                           \
+    else if (s.lanes == 64) { GO(64, 2, 256); }                                        \
+    else if (s.lanes == 256 && s.nv == 1) { GO(256, 1, 256); }                         \
+    else if (s.lanes == 256) { GO(256, 2, 256); }                                      \
+    else if (s.nv == 1) { GO(1024, 1, 1024); }                                         \
+    else { GO(1024, 2, 1024); }                                                        \
+  } while (0)
 
 template <typename T, typename P>
 void launch_fwd(const NormArgs &a) {
@@ -409,12 +417,15 @@ void launch_fwd(const NormArgs &a) {
   long long g = (a.m + groups - 1) / groups;
   const long long most = s.threads == 1024 ? 512 : 2048;      // every workgroup resident
   const int grid = (int)(g < most ? g : most);
-#define SF_GO(L, N, TH)                                                                        \
-  hipLaunchKernelGGL((norm_fwd_kernel<T, P, L, N, TH>), dim3(grid), dim3(TH), 0, a.st,         \
+  const bool nt = (size_t)a.m * a.d * sizeof(T) >= kSfStreamBytes;
+#define SF_GO1(L, N, TH, NT)                                                                   \
+  hipLaunchKernelGGL((norm_fwd_kernel<T, P, L, N, TH, NT>), dim3(grid), dim3(TH), 0, a.st,     \
                      (const T *)a.x, (const T *)a.res, a.w, a.b, (T *)a.y, (T *)a.sum, a.mean, \
                      a.rstd, a.m, a.d, a.eps)
+#define SF_GO(L, N, TH) if (nt && TH == 256) SF_GO1(L, N, TH, (TH == 256)); else SF_GO1(L, N, TH, false)
   SF_NORM_SHAPES(SF_GO);
 #undef SF_GO
+#undef SF_GO1
 }
 
 template <typename T, typename P>
@@ -431,13 +442,16 @@ void launch_bwd(const NormArgs &a) {
                          a.part, a.m, a.d);
     return;
   }
-#define SF_GO(L, N, TH)                                                                            \
-  hipLaunchKernelGGL((norm_bwd_kernel<T, P, L, N, TH>), dim3(a.blocks), dim3(TH),                  \
+  const bool nt = (size_t)a.m * a.d * sizeof(T) >= kSfStreamBytes;
+#define SF_GO1(L, N, TH, NT)                                                                       \
+  hipLaunchKernelGGL((norm_bwd_kernel<T, P, L, N, TH, NT>), dim3(a.blocks), dim3(TH),              \
                      TH == L ? 0 : (size_t)TH * N * SfChunk<T>::V * sizeof(float), a.st,           \
                      (const T *)a.dy, (const T *)a.x, a.mean, a.rstd, a.w, (const T *)a.sum,       \
                      (T *)a.y, a.part, a.m, a.d)
+#define SF_GO(L, N, TH) if (nt && TH == 256) SF_GO1(L, N, TH, (TH == 256)); else SF_GO1(L, N, TH, false)
   SF_NORM_SHAPES(SF_GO);
 #undef SF_GO
+#undef SF_GO1
 }
 
 template <typename T>

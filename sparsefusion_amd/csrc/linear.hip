@@ -144,7 +144,7 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
 // A workgroup owns 32 chunks of columns and a run of rows, 8 row lanes deep; dz goes out as it is
 // computed, the column sums stay in registers, join through LDS and leave as part[run][n].  The sums
 // are of the fp32 products, not of the rounded dz.
-template <typename T>
+template <typename T, bool NT>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
           float *__restrict__ part, long long m, long long n, long long run) {
@@ -163,8 +163,8 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
         const long long row = r + 8 * i < r1 ? r + 8 * i : r;
-        sf_load_chunk<T>(dy + row * n, col, n, g[i]);
-        if (act != SF_ACT_NONE) sf_load_chunk<T>(pre + row * n, col, n, z[i]);
+        sf_load_chunk<T, NT>(dy + row * n, col, n, g[i]);
+        if (act != SF_ACT_NONE) sf_load_chunk<T, NT>(pre + row * n, col, n, z[i]);
       }
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
@@ -218,7 +218,8 @@ void run_dz(const void *dy, const void *pre, int act, void *dz, SfColumnSums &db
   const long long run = (m + want - 1) / want;
   db.part = part, db.n = n, db.runs = (int)((m + run - 1) / run);
   const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), db.runs);
-  hipLaunchKernelGGL((dz_kernel<T>), grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act, (T *)dz,
+  auto kern = (size_t)m * n * sizeof(T) >= kSfStreamBytes ? dz_kernel<T, true> : dz_kernel<T, false>;
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act, (T *)dz,
                      padded(n, dtype), db.out ? part : nullptr, m, n, run);
 }
 void join_db(const SfColumnSums &db, int dtype, hipStream_t st) {
