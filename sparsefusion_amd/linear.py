@@ -25,19 +25,20 @@ def _act_code(activation):
     return code
 
 
-def _check(x, weight):
+def _check(x, weight, device):
     """-> (n, k, dtype code) of a well-formed pair."""
-    code = _lib.DTYPE_CODES.get(x.dtype)
+    dtype = x.dtype
+    code = _lib.DTYPE_CODES.get(dtype)
     if code is None:
-        raise RuntimeError(f'linear takes fp32, fp16 or bf16, got {x.dtype}')
+        raise RuntimeError(f'linear takes fp32, fp16 or bf16, got {dtype}')
     if weight.dim() != 2:
         raise RuntimeError(f'weight must be (out_features, in_features), got {tuple(weight.shape)}')
     n, k = weight.shape
     if x.dim() < 1 or x.shape[-1] != k:
         raise RuntimeError(f'expected rows of {k} elements, got {tuple(x.shape)}')
-    if max(n, k) > MOST_FEATURES:
+    if n > MOST_FEATURES or k > MOST_FEATURES:
         raise RuntimeError(f'linear takes up to {MOST_FEATURES} features, got {k} -> {n}')
-    if weight.dtype != x.dtype or weight.device != x.device:
+    if weight.dtype != dtype or weight.device != device:
         _lib.same(x, 'weight', weight)
     return n, k, code
 
@@ -46,39 +47,43 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     """-> (y, pre): y = act(x @ weight.T + bias) + residual and, with keep_pre, the values before
     the activation (None otherwise).  x (..., K), weight (N, K), bias (N,), residual (..., N) or
     anything that expands to it.  Not differentiable: see `linear`."""
-    act = _act_code(activation)
-    n, k, code = _check(x, weight)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        act = _act_code(activation)
+    device = x.device
+    n, k, code = _check(x, weight, device)
     shape = (x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n)
+    pb = pr = pp = None
     if bias is not None:
-        if bias.dtype != x.dtype or bias.device != x.device:
-            _lib.same(x, 'bias', bias)
+        _lib.same(x, 'bias', bias)
         if bias.dim() != 1 or bias.shape[0] != n:
             raise RuntimeError(f'bias must have shape ({n},), got {tuple(bias.shape)}')
         bias = bias.contiguous()
+        pb = bias.data_ptr()
     if residual is not None:
         _lib.same(x, 'residual', residual)
         if residual.shape != shape:
             residual = residual.expand(shape)
         residual = residual.contiguous()
-    if _lib.elsewhere(x.device):
-        with torch.cuda.device(x.device):
+        pr = residual.data_ptr()
+    if _lib.elsewhere(device):
+        with torch.cuda.device(device):
             return linear_forward(x, weight, bias, activation, residual, keep_pre)
     rows, ldx = _lib.rows(x)
-    m = rows.shape[0]
     weight = weight.contiguous()
     y = x.new_empty(shape)
-    pre = x.new_empty(shape) if keep_pre else None
+    pre = None
+    if keep_pre:
+        pre = x.new_empty(shape)
+        pp = pre.data_ptr()
+    m, px, pw, py, stream = rows.shape[0], rows.data_ptr(), weight.data_ptr(), y.data_ptr(), _lib.stream(device)
     L = _lib.lib()
-    px, pw = rows.data_ptr(), weight.data_ptr()
-    args = (px, ldx, pw, None if bias is None else bias.data_ptr(),
-            None if residual is None else residual.data_ptr(), y.data_ptr(),
-            None if pre is None else pre.data_ptr(), m, k, n, code, act)
     # most sizes need no scratch: only a refusal asks how much
-    rc = L.sf_linear(*args, None, 0, _lib.stream(x.device))
+    rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, None, 0, stream)
     if rc == _lib.SF_ERR_WORKSPACE:
         nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
-        rc = L.sf_linear(*args, ws.data_ptr(), nbytes, _lib.stream(x.device))
+        rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, ws.data_ptr(), nbytes, stream)
     if rc:
         _lib.check(rc)
     return y, pre
@@ -89,7 +94,7 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     output; `pre` as it returned them (not needed without an activation).  `needs` says which are
     wanted, the others are None.  The residual's gradient is `grad` itself."""
     act = _act_code(activation)
-    n, k, code = _check(x, weight)
+    n, k, code = _check(x, weight, x.device)
     shape = (*x.shape[:-1], n)
     if not act:
         pre = None
