@@ -12,9 +12,10 @@
 //
 // A workgroup owns a BP x BQ tile and walks k in steps of 128 bytes (64 16-bit or 32 fp32 elements).
 // Both operands' tiles go to LDS in 16-byte chunks straight from memory (buffer_load ... lds), into a
-// ring of buffers up to three steps ahead.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32; Q is the instruction's first
-// operand, so a lane ends up with four consecutive q of one row p.  Workgroups stay and walk the
-// tiles: the loads of the next tile's first steps run under the epilogue of the last.
+// ring of buffers up to three steps ahead.  v_mfma_f32_32x32x16 (32x32x2 for fp32) accumulates in fp32;
+// Q is the instruction's first operand, so a lane ends up with four consecutive q of one row p.
+// Workgroups stay and walk the tiles: the loads of the next tile's first steps run under the epilogue of
+// the last.
 // Rows and k outside the operands read as zeros (the buffer descriptor's range check), columns
 // outside are never stored.
 //
@@ -142,7 +143,8 @@ struct SfOperand {
   static __device__ __forceinline__ int swz(int row) {
     if constexpr (!KMINOR && STEP == 128) return (row ^ (row >> 3)) & 7;
     else if constexpr (!KMINOR) return (row >> 3) & 3;
-    else if constexpr (S == 4) return ((row >> 2) & 1) << 3;
+    else if constexpr (S == 4) return CPR == 8 ? 0 : ((row >> 2) & 1) << 3;
+    else if constexpr (CPR == 4) return 0;
     else if constexpr (CPR == 8) return ((row >> 1) & 1) << 2;
     else return (row & 3) << 2;
   }
@@ -670,17 +672,132 @@ static void sf_gemm_join(const SfGemmArgs &a, hipStream_t st) {
 }
 
 // The launches of one storage type (linear_f32.hip, linear_f16.hip, linear_bf16.hip).
-// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.  tile 64, 128 or 256, operands as sf_whole_chunks
-// says; layout 0 only: SF_FEW_ROWS, any operands.
+// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.  tile 32, 64, 128 or 256, operands of whole
+// aligned 16-byte chunks; layout 0 only: SF_FEW_ROWS, any operands.
 #define SF_FEW_ROWS 16
 int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
-// Both gradients' products, 64 x 64 tiles without splits, and the bias gradient's sum.
+// Both gradients' products, 32 x 32 tiles, and the bias gradient's sum.
 struct SfColumnSums;
 int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
+
+// ---- small products -------------------------------------------------------------------------------
+// Too few 64 x 64 tiles to fill the chip leave each CU with one workgroup that walks a long contraction
+// alone.  Here a workgroup owns 32 x 32 outputs and its four waves share each step's 128 bytes of k, 32
+// each, so a step takes a quarter of the products' time; a ring of eight buffers keeps seven steps in
+// flight.  The waves' sums meet in LDS.  In us, 64 x 64 tiles against these: 200 x 128 -> 256 fp32 5.9 and
+// 4.3, 400 x 1024 -> 256 bf16 7.8 and 5.6 (fp32 23 and 10), 1000 x 512 -> 512 fp32 14 and 10.3; twice the
+// operand bytes per output loses once the chip is full (2000 x 512 -> 512 fp32 15.0 and 19.6).
+struct SfSmall {
+  static constexpr int B = 32, STEP = 128, RING = 8, BYTES = 2 * B * STEP, LDS = RING * BYTES;
+};
+
+template <typename T, bool PMINOR, bool QMINOR>
+__device__ __forceinline__ void sf_small(const SfGemmArgs &a, unsigned char *lds, int group) {
+  constexpr int B = SfSmall::B, STEP = SfSmall::STEP, RING = SfSmall::RING, BYTES = SfSmall::BYTES;
+  constexpr int V = 16 / sizeof(T), BK = STEP / (int)sizeof(T);
+  typedef SfOperand<T, PMINOR, B, 4, STEP> OP;
+  typedef SfOperand<T, QMINOR, B, 4, STEP> OQ;
+  typedef typename SfMfma<T>::frag frag;
+  constexpr int NI = OP::NI + OQ::NI;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#if defined(__HIP_DEVICE_COMPILE__)
+  const unsigned lds0 = (unsigned)(unsigned long long)(__attribute__((address_space(3))) unsigned char *)lds;
+#else
+  const unsigned lds0 = 0;
+#endif
+  const int split = group / (a.tiles_p * a.tiles_q), tile = group - split * (a.tiles_p * a.tiles_q);
+  const long long p0 = (long long)(tile / a.tiles_q) * B, q0 = (long long)(tile % a.tiles_q) * B;
+  const long long k0 = split * a.k_split;
+  const int steps = sf_steps<BK>(a, split);
+  const long long left = a.nk - k0 - (long long)(steps - 1) * BK;
+  const int last_k = left < BK ? (int)left : BK;
+  OP op;
+  OQ oq;
+  op.init(a.ldp, wave, lane);
+  oq.init(a.ldq, wave, lane);
+  op.open(a.p, p0, a.np, k0, steps, last_k);
+  oq.open(a.q, q0, a.nq, k0, steps, last_k);
+  auto load = [&](int buf) {      // behind the last step: loads of nothing, so that the counted waits hold
+    sf_unroll<0, OP::NI>([&](auto j) { op.template issue<decltype(j)::value>(lds0 + buf + wave * 1024); });
+    sf_unroll<0, OQ::NI>([&](auto j) {
+      oq.template issue<decltype(j)::value>(lds0 + buf + B * STEP + wave * 1024);
+    });
+    op.next(), oq.next();
+    if (op.steps == 0) op.close(), oq.close();
+  };
+#pragma unroll
+  for (int i = 0; i + 1 < RING; ++i) load(i * BYTES);
+  sf_f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+  int cur = 0, old = (RING - 1) * BYTES;
+  for (int i = 0; i < steps; ++i) {
+    asm volatile("" ::: "memory");
+    sf_wait_loads<(RING - 2) * NI>();
+    __builtin_amdgcn_s_barrier();      // step i has landed, everyone has read step i - 1
+    asm volatile("" ::: "memory");
+    const frag fp = OP::fragment(lds + cur, 0, wave, lane);
+    const frag fq = OQ::fragment(lds + cur + B * STEP, 0, wave, lane);
+    load(old);
+    acc = SfMfma<T>::run(fq, fp, acc);
+    old = cur;
+    cur = cur + BYTES == RING * BYTES ? 0 : cur + BYTES;
+  }
+  sf_wait_loads<0>();
+  __syncthreads();
+  // lane (row = lane % 32, h = lane / 32) holds columns 8 g + 4 h + 0..3: the waves' blocks behind each
+  // other, quads swizzled by the row
+  float *part = reinterpret_cast<float *>(lds);
+  const int row = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<sf_f32x4 *>(part + wave * 1024 + row * 32 + (((2 * g + h) ^ row ^ (row >> 3)) & 7) * 4) =
+        (sf_f32x4){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  __syncthreads();
+  const int r = threadIdx.x >> 3, quad = threadIdx.x & 7;      // 32 rows by 8 quads
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const sf_f32x4 f =
+        *reinterpret_cast<const sf_f32x4 *>(part + w * 1024 + r * 32 + ((quad ^ r ^ (r >> 3)) & 7) * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += f[j];
+  }
+  const long long prow = p0 + r, col = q0 + 4 * quad;
+  if (prow < a.np) {
+    const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
+    T *out = static_cast<T *>(a.out), *pre = static_cast<T *>(a.pre);
+    const long long at = prow * a.nq + col;
+    if (a.splits > 1) {
+      if (col < a.nq) sf_store_chunk<float>(a.partial + ((long long)split * a.np + prow) * a.nq, col, a.nq, v);
+      return;
+    }
+    float b[4], x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {      // columns past the end read the last one's
+      const long long c = col + j < a.nq ? j : a.nq - 1 - col;
+      b[j] = bias ? (float)bias[col + c] : 0.0f;
+      x[j] = res ? (float)res[at + c] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + j < a.nq) {
+        const float z = v[j] + b[j];
+        if (pre) pre[at + j] = (T)z;
+        out[at + j] = (T)(sf_act<T>(z, a.act) + x[j]);
+      }
+  }
+}
+
+template <typename T, bool PMINOR, bool QMINOR>
+__global__ void __launch_bounds__(256) sf_small_kernel(SfGemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[SfSmall::LDS];
+  sf_small<T, PMINOR, QMINOR>(a, lds, blockIdx.x);
+}
 
 template <typename T, bool PMINOR, bool QMINOR, typename SH>
 static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
@@ -709,7 +826,11 @@ typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64Three;
 template <typename T, bool PMINOR, bool QMINOR>
 static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
   int rc;
-  if (tile == 256) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
+  if (tile == 32) {
+    hipLaunchKernelGGL((sf_small_kernel<T, PMINOR, QMINOR>), dim3(a.tiles_p * a.tiles_q * a.splits), dim3(256),
+                       0, st, a);
+    rc = SF_OK;
+  } else if (tile == 256) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
   else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
   else if (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
   else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
@@ -750,15 +871,17 @@ __device__ __forceinline__ void sf_join_columns(const SfColumnSums &c, int group
   }
 }
 
-// dx = dz w, dw = dz^T x and db's last sum by different workgroups of one launch: products of a few tiles
-// each are all latency (400 x 256 -> 128 fp32: 7 us each, one behind the other, and a launch more).
-template <typename T, typename SH>
-__global__ void __launch_bounds__(SH::WAVES * 64, SH::WGS * SH::WAVES / 4)
+// dx = dz w, dw = dz^T x and db's last sum by different workgroups of one launch, the longest first:
+// products of a few tiles each are all latency.  400 x 256 -> 128 with the pass for dz in front: fp32
+// 10.0 us, bf16 10.3 (64 x 64 tiles in one launch 16.9, one product behind the other 21);
+// 1000 x 512 -> 512 bf16 17.9 (26).
+template <typename T>
+__global__ void __launch_bounds__(256)
 sf_gradients_kernel(SfGemmArgs dx, int dx_groups, SfGemmArgs dw, int dw_groups, SfColumnSums db) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[SH::LDS];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[SfSmall::LDS];
   const int g = blockIdx.x;
-  if (g < dx_groups) sf_gemm<T, false, true, SH>(dx, lds, g, dx_groups);
-  else if (g < dx_groups + dw_groups) sf_gemm<T, true, true, SH>(dw, lds, g - dx_groups, dw_groups);
+  if (g < dw_groups) sf_small<T, true, true>(dw, lds, g);
+  else if (g < dx_groups + dw_groups) sf_small<T, false, true>(dx, lds, g - dw_groups);
   else sf_join_columns<T>(db, g - dx_groups - dw_groups, reinterpret_cast<float *>(lds));
 }
 
@@ -766,8 +889,7 @@ template <typename T>
 static int sf_gradients_go(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
   const int nx = dx.tiles_p * dx.tiles_q, nw = dw.tiles_p * dw.tiles_q;
   const int nb = db.out ? (int)((db.n + 31) / 32) : 0;
-  hipLaunchKernelGGL((sf_gradients_kernel<T, SfTile64Three>), dim3(nx + nw + nb), dim3(256), 0, st, dx, nx, dw,
-                     nw, db);
+  hipLaunchKernelGGL((sf_gradients_kernel<T>), dim3(nx + nw + nb), dim3(256), 0, st, dx, nx, dw, nw, db);
   return SF_OK;
 }
 

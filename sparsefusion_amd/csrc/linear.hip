@@ -9,21 +9,36 @@ namespace {
 struct Plan {
   int tile, splits;
   long long k_split;
+  double cost;
 };
 
-// Tile and splits of a np x nq product over nk: the cheapest of the three tiles, each whole or with the
-// contraction cut into as many parts as fill the chip, by a model of the busiest CU (us; per step of
-// 128 bytes of k, fitted to 20 sizes from 1 x 1024 x 4096 to 8192^3).
+// Time (us, without the launch) of t workgroups of a tile's kernel, each `per` steps of 128 bytes of k,
+// on the busiest CU; fitted to 30 sizes from 64 x 64 x 64 to 8192^3.  Two 128 x 128 tiles share a CU and
+// take hardly longer than one.
+double tile_cost(int tile, long long t, long long per, int dtype) {
+  const double n = (double)((t + 255) / 256), k = (double)per;
+  if (dtype == SF_DTYPE_F32)
+    return tile == 256   ? n * (8 + 7.5 * k)
+           : tile == 128 ? n * (2 + 2.05 * k)
+           : tile == 64  ? n * (0.7 + (n < 2 ? 0.7 : 0.57) * k)
+                         : n * (0.3 + 0.24 * k);
+  return tile == 256   ? n * (8 + 1.75 * k)
+         : tile == 128 ? (double)((t + 511) / 512) * (4 + k)
+         : tile == 64  ? n * (0.8 + 0.3 * k)
+                       : n * (0.3 + 0.165 * k);
+}
+
+// Tile and splits of a np x nq product over nk: the cheapest of the four tiles, each whole or with the
+// contraction cut into as many parts as fill the chip.
 Plan make_plan(long long np, long long nq, long long nk, int dtype) {
   const long long bk = 128 / (long long)sf_dtype_size(dtype);
   const long long steps = (nk + bk - 1) / bk;
-  Plan best{128, 1, steps * bk};
+  Plan best{128, 1, steps * bk, 1e30};
   if (np < 1 || nq < 1 || nk < 1) return best;      // no product
-  double least = 1e30;
-  for (int tile : {256, 128, 64}) {
+  for (int tile : {256, 128, 64, 32}) {
     const long long t = ((np + tile - 1) / tile) * ((nq + tile - 1) / tile);
     for (int full = 0; full < 2; ++full) {
-      const int slots = 256 * (tile == 256 ? 1 : tile == 128 ? 2 : 3);
+      const int slots = 256 * (tile == 256 ? 1 : tile == 64 ? 3 : 2);
       long long s = 1;
       if (full) {
         s = slots / t < steps / 4 ? slots / t : steps / 4;
@@ -31,13 +46,9 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype) {
       }
       const long long per = (steps + s - 1) / s;
       s = (steps + per - 1) / per;
-      const long long n = (t * s + 255) / 256;      // workgroups of the busiest CU, one after the other but:
-      const double pairs = (double)((n + 1) / 2);   // two 128 tiles take hardly longer than one
-      double c = dtype == SF_DTYPE_F32
-                     ? n * (tile == 256 ? 8 + 7.5 * per : tile == 128 ? 2 + 2.05 * per : 0.7 + 0.57 * per)
-                     : tile == 256 ? n * (8 + 1.75 * per) : tile == 128 ? pairs * (4 + per) : n * (0.8 + 0.3 * per);
+      double c = tile_cost(tile, t * s, per, dtype);
       if (s > 1) c += 6 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
-      if (c < least) least = c, best = Plan{tile, (int)s, per * bk};
+      if (c < best.cost) best = Plan{tile, (int)s, per * bk, c};
     }
   }
   return best;
@@ -241,6 +252,7 @@ int zero_out(void *p, long long elements, int dtype, hipStream_t st) {
 // Where the pieces of the backward pass's workspace start, and what is copied first.
 struct BackwardPlan {
   Plan dx, dw;
+  bool pair;      // both products in one launch
   bool write_dz, pack_x, pack_w;
   size_t dz, x, w, part, split, bytes;
 };
@@ -249,6 +261,17 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   BackwardPlan b;
   b.dx = make_plan(m, k, n, dtype);
   b.dw = make_plan(n, k, m, dtype);
+  auto small = [&](long long np, long long nq, long long nk) {
+    const long long bk = 128 / (long long)sf_dtype_size(dtype), steps = (nk + bk - 1) / bk;
+    const long long t = ((np + 31) / 32) * ((nq + 31) / 32);
+    return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype)};
+  };
+  // One launch for both products in 32 x 32 tiles where that is cheaper than two: a launch costs the host
+  // 3 us, and one product runs in the other's idle CUs.  With one of the two gradients asked for the
+  // tiles stay the same, so that its values do.
+  const Plan x32 = small(m, k, n), w32 = small(n, k, m);
+  b.pair = k > 0 && x32.cost + w32.cost < 100 && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
+  if (b.pair) b.dx = x32, b.dw = w32;
   b.write_dz = act != SF_ACT_NONE || !whole_chunks(dy, n, n, dtype);
   b.pack_x = !whole_chunks(x, ldx, k, dtype);
   b.pack_w = !whole_chunks(w, k, k, dtype);
@@ -325,7 +348,7 @@ extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const
   a.np = m, a.nq = n, a.nk = k;
   a.bias = bias, a.residual = residual, a.out = y, a.pre = pre;
   a.act = act;
-  if (k == 0) return product(a, 0, dtype, make_plan(m, n, k, dtype), st);
+  if (k == 0) return product(a, 0, dtype, Plan{128, 1, 0, 0}, st);
   const ForwardPlan f = forward_plan(x, ldx, weight, m, k, n, dtype);
   if (f.few) return launch(a, 0, dtype, SF_FEW_ROWS, st);
   SF_LINEAR_CHECK_WORKSPACE("sf_linear", f.bytes);
@@ -388,10 +411,9 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   gw.np = n, gw.nq = k, gw.nk = m;
   gw.out = dw;
   gx.partial = gw.partial = (float *)(base + b.split);
-  // one launch while every workgroup of both products is resident at once
-  if (dx && dw && b.dx.tile == 64 && b.dw.tile == 64 && b.dx.splits == 1 && b.dw.splits == 1 &&
-      prepare(gx, b.dx) && prepare(gw, b.dw) &&
-      (long long)gx.tiles_p * gx.tiles_q + (long long)gw.tiles_p * gw.tiles_q <= 768) {
+  if (dx && dw && b.pair) {
+    prepare(gx, b.dx);
+    prepare(gw, b.dw);
     rc = dtype == SF_DTYPE_F32   ? sf_gradients_f32(gx, gw, sums, st)
          : dtype == SF_DTYPE_F16 ? sf_gradients_f16(gx, gw, sums, st)
                                  : sf_gradients_bf16(gx, gw, sums, st);
