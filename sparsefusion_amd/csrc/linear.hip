@@ -22,7 +22,7 @@ double tile_cost(int tile, long long t, long long per, int dtype) {
            : tile == 128 ? n * (2 + 2.05 * k)
            : tile == 64  ? n * (0.7 + (n < 2 ? 0.7 : 0.57) * k)
                          : n * (0.3 + 0.24 * k);
-  return tile == 256   ? n * (8 + 1.75 * k)
+  return tile == 256   ? n * (11 + 1.75 * k)
          : tile == 128 ? (double)((t + 511) / 512) * (4 + k)
          : tile == 64  ? n * (0.8 + 0.3 * k)
                        : n * (0.3 + 0.165 * k);
