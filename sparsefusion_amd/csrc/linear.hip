@@ -28,6 +28,11 @@ double tile_cost(int tile, long long t, long long per, int dtype) {
                        : n * (0.3 + 0.165 * k);
 }
 
+// 32 x 32 tiles only as long as all of them are resident, two to a CU: a workgroup there walks one tile,
+// and its start and first loads show in every further round (100000 x 64 -> 32 bf16: 22.6 us, with
+// 64 x 64 tiles 11.4; 5000 x 256 -> 64 fp32, 314 tiles: 7.6 and 8.9).
+constexpr long long kMostSmallTiles = 512;
+
 // Tile and splits of a np x nq product over nk: the cheapest of the four tiles, each whole or with the
 // contraction cut into as many parts as fill the chip.
 Plan make_plan(long long np, long long nq, long long nk, int dtype) {
@@ -46,6 +51,7 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype) {
       }
       const long long per = (steps + s - 1) / s;
       s = (steps + per - 1) / per;
+      if (tile == 32 && t * s > kMostSmallTiles) continue;
       double c = tile_cost(tile, t * s, per, dtype);
       if (s > 1) c += 6 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
       if (c < best.cost) best = Plan{tile, (int)s, per * bk, c};
@@ -152,41 +158,41 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
 }
 
 // ---- dz and the bias gradient -------------------------------------------------------------------
-// A workgroup owns 32 chunks of columns and a run of rows, 8 row lanes deep; dz goes out as it is
-// computed, the column sums stay in registers, join through LDS and leave as part[run][n].  The sums
-// are of the fp32 products, not of the rounded dz.
-template <typename T, bool NT>
+// A workgroup owns CL chunks of columns (32, fewer for narrow layers) and a run of rows, 256 / CL at a
+// time; dz goes out as it is computed, the column sums stay in registers, join through LDS and leave as
+// part[run][n].  The sums are of the fp32 products, not of the rounded dz.
+template <typename T, int CL, bool NT>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
           float *__restrict__ part, long long m, long long n, long long run) {
-  constexpr int V = 16 / sizeof(T), DEEP = 4;
-  __shared__ float red[8][32 * V + 4];
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const long long col = ((long long)blockIdx.x * 32 + cl) * V;
+  constexpr int V = 16 / sizeof(T), DEEP = 4, RL = 256 / CL;
+  __shared__ float red[RL][CL * V + 4];
+  const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
+  const long long col = ((long long)blockIdx.x * CL + cl) * V;
   const long long r0 = blockIdx.y * run, r1 = r0 + run < m ? r0 + run : m;
   float sum[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.0f;
   if (col < n)
-    for (long long r = r0 + rl; r < r1; r += 8 * DEEP) {
+    for (long long r = r0 + rl; r < r1; r += RL * DEEP) {
       // DEEP rows' loads in flight; rows past the run are read again and count for nothing
       float g[DEEP][V], z[DEEP][V];
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
-        const long long row = r + 8 * i < r1 ? r + 8 * i : r;
+        const long long row = r + RL * i < r1 ? r + RL * i : r;
         sf_load_chunk<T, NT>(dy + row * n, col, n, g[i]);
         if (act != SF_ACT_NONE) sf_load_chunk<T, NT>(pre + row * n, col, n, z[i]);
       }
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
-        if (r + 8 * i >= r1) break;
+        if (r + RL * i >= r1) break;
         if (act != SF_ACT_NONE) {
 #pragma unroll
           for (int j = 0; j < V; ++j) g[i][j] *= sf_act_slope<T>(z[i][j], act);
         }
         // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a
         // ReLU's or GELU's gradient of zero is zero
-        if (dz) sf_store_chunk<T>(dz + (r + 8 * i) * ldz, col, ldz, g[i]);
+        if (dz) sf_store_chunk<T>(dz + (r + RL * i) * ldz, col, ldz, g[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] += g[i][j];
       }
@@ -195,28 +201,33 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
 #pragma unroll
   for (int j = 0; j < V; ++j) red[rl][cl * V + j] = sum[j];
   __syncthreads();
-  for (int i = threadIdx.x; i < 32 * V; i += 256) {
-    const long long c = (long long)blockIdx.x * 32 * V + i;
+  for (int i = threadIdx.x; i < CL * V; i += 256) {
+    const long long c = (long long)blockIdx.x * CL * V + i;
     if (c >= n) break;
     float t = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][i];
+    for (int k = 0; k < RL; ++k) t += red[k][i];
     part[(long long)blockIdx.y * n + c] = t;
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) db_join_kernel(SfColumnSums c) {
-  __shared__ float red[8 * 33];
-  sf_join_columns<T>(c, blockIdx.x, red);
+template <typename T, int TY>
+__global__ void __launch_bounds__(32 * TY) db_join_kernel(SfColumnSums c) {
+  __shared__ float red[TY * 33];
+  sf_join_columns<T, TY>(c, blockIdx.x, red);
 }
 
-// Runs of rows of dz_kernel: about 2048 workgroups in all, at least 32 rows each.
+// Chunks of columns to a workgroup of dz_kernel, and its runs of rows: about 2048 workgroups in all, at
+// least four turns of rows each.  (259200 x 64 bf16: 29 us with 8 chunks, 66 with 32.)
+int dz_chunks(long long n, int dtype) {
+  const long long v = 16 / (long long)sf_dtype_size(dtype), chunks = (n + v - 1) / v;
+  return chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
+}
 int dz_runs(long long m, long long n, int dtype) {
-  const long long v = 16 / (long long)sf_dtype_size(dtype);
-  const long long strips = (n + 32 * v - 1) / (32 * v);
+  const long long v = 16 / (long long)sf_dtype_size(dtype), cl = dz_chunks(n, dtype);
+  const long long strips = (n + cl * v - 1) / (cl * v), least = 4 * 256 / cl;
   long long runs = (2048 + strips - 1) / strips;
-  if (runs > (m + 31) / 32) runs = (m + 31) / 32;
+  if (runs > (m + least - 1) / least) runs = (m + least - 1) / least;
   return (int)(runs < 1 ? 1 : runs);
 }
 
@@ -225,19 +236,23 @@ template <typename T>
 void run_dz(const void *dy, const void *pre, int act, void *dz, SfColumnSums &db, float *part, long long m,
             long long n, int dtype, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int want = dz_runs(m, n, dtype);
+  const int want = dz_runs(m, n, dtype), cl = dz_chunks(n, dtype);
   const long long run = (m + want - 1) / want;
   db.part = part, db.n = n, db.runs = (int)((m + run - 1) / run);
-  const dim3 grid((unsigned)((n + 32 * V - 1) / (32 * V)), db.runs);
-  auto kern = (size_t)m * n * sizeof(T) >= kSfStreamBytes ? dz_kernel<T, true> : dz_kernel<T, false>;
+  const dim3 grid((unsigned)((n + cl * V - 1) / (cl * V)), db.runs);
+  const bool nt = (size_t)m * n * sizeof(T) >= kSfStreamBytes;
+  auto kern = cl == 8    ? nt ? dz_kernel<T, 8, true> : dz_kernel<T, 8, false>
+              : cl == 16 ? nt ? dz_kernel<T, 16, true> : dz_kernel<T, 16, false>
+                         : nt ? dz_kernel<T, 32, true> : dz_kernel<T, 32, false>;
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act, (T *)dz,
                      padded(n, dtype), db.out ? part : nullptr, m, n, run);
 }
-void join_db(const SfColumnSums &db, int dtype, hipStream_t st) {
+// The sum that the products' launch would have made (`pair`: in the same order), or a deeper one.
+template <typename T>
+void join_db(const SfColumnSums &db, bool pair, hipStream_t st) {
   const dim3 grid(sf_div_up(db.n, 32));
-  if (dtype == SF_DTYPE_F32) hipLaunchKernelGGL((db_join_kernel<float>), grid, dim3(256), 0, st, db);
-  else if (dtype == SF_DTYPE_F16) hipLaunchKernelGGL((db_join_kernel<_Float16>), grid, dim3(256), 0, st, db);
-  else hipLaunchKernelGGL((db_join_kernel<__bf16>), grid, dim3(256), 0, st, db);
+  if (pair) hipLaunchKernelGGL((db_join_kernel<T, 8>), grid, dim3(256), 0, st, db);
+  else hipLaunchKernelGGL((db_join_kernel<T, 32>), grid, dim3(1024), 0, st, db);
 }
 
 int zero_out(void *p, long long elements, int dtype, hipStream_t st) {
@@ -270,7 +285,7 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   // 3 us, and one product runs in the other's idle CUs.  With one of the two gradients asked for the
   // tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
-  b.pair = k > 0 && x32.cost + w32.cost < 100 && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
+  b.pair = k > 0 && m < (1 << 20) && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
   if (b.pair) b.dx = x32, b.dw = w32;
   b.write_dz = act != SF_ACT_NONE || !whole_chunks(dy, n, n, dtype);
   b.pack_x = !whole_chunks(x, ldx, k, dtype);
@@ -422,7 +437,9 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
     return SF_OK;
   }
   if (db) {
-    join_db(sums, dtype, st);
+    if (dtype == SF_DTYPE_F32) join_db<float>(sums, b.pair, st);
+    else if (dtype == SF_DTYPE_F16) join_db<_Float16>(sums, b.pair, st);
+    else join_db<__bf16>(sums, b.pair, st);
     SF_CHECK_LAUNCH();
   }
   if (dx && (rc = product(gx, 1, dtype, b.dx, st))) return rc;
