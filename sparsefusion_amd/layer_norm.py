@@ -164,9 +164,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, return_sum=Fa
     return (y, s) if return_sum else y
 
 
-@NORM_LAYERS.register_module('LN')
 class LayerNorm(nn.LayerNorm):
     """`nn.LayerNorm` over the last dimension with an optional residual added in front."""
+
+    _abbr_ = 'ln'
 
     def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, device=None,
                  dtype=None):
@@ -179,3 +180,7 @@ class LayerNorm(nn.LayerNorm):
             raise RuntimeError(f'expected rows of {self.normalized_shape[0]} elements, got '
                                f'{tuple(x.shape)}')
         return layer_norm(x, self.weight, self.bias, self.eps, residual, return_sum)
+
+
+if NORM_LAYERS.get('LN') is None:
+    NORM_LAYERS.register_module('LN', module=LayerNorm)

@@ -58,10 +58,13 @@ def build_conv_layer(cfg, *args, **kwargs):
 
 
 def build_norm_layer(cfg, num_features, postfix=''):
-    """mmcv.cnn.build_norm_layer -> (name, layer); abbreviations 'bn' and 'ln' as mmcv infers them."""
-    from . import layer_norm  # noqa: F401  (registers LN)
+    """mmcv.cnn.build_norm_layer -> (name, layer); abbreviation 'bn' as mmcv infers for BN*, 'ln' for
+    LN (its `_abbr_`)."""
     cfg = dict(cfg)
-    cls = NORM_LAYERS.get(cfg.pop('type'))
+    kind = cfg.pop('type')
+    cls = NORM_LAYERS.get(kind)
+    if cls is None and kind == 'LN':      # registers itself; a caller's own LN keeps the name
+        from .layer_norm import LayerNorm as cls
     if cls is None:
         raise KeyError('unknown norm layer type')
     requires_grad = cfg.pop('requires_grad', True)
@@ -69,7 +72,7 @@ def build_norm_layer(cfg, num_features, postfix=''):
     layer = cls(num_features, **cfg)
     for p in layer.parameters():
         p.requires_grad = requires_grad
-    return ('ln' if isinstance(layer, nn.LayerNorm) else 'bn') + str(postfix), layer
+    return getattr(layer, '_abbr_', 'bn') + str(postfix), layer
 
 
 def build_linear_layer(cfg, *args, **kwargs):

@@ -49,8 +49,8 @@ class VFELayer(nn.Module):
         self.cat_max = cat_max
         self.max_out = max_out
         self.norm = build_norm_layer(norm_cfg, out_channels)[1]
-        if not isinstance(self.norm, nn.BatchNorm1d):
-            raise NotImplementedError(f'norm layer {norm_cfg} (the kernel folds an eval BatchNorm1d)')
+        if not hasattr(self.norm, 'running_mean'):
+            raise NotImplementedError(f'norm layer {norm_cfg} (the kernel folds an eval BatchNorm)')
         self.linear = nn.Linear(in_channels, out_channels, bias=False)
 
     def _run(self, inputs, decorate=0, num_points=None, coors=None, voxel_size=None, pc_range=None):

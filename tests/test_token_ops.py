@@ -173,8 +173,28 @@ def test_refusals_need_no_device():
     with pytest.raises(NotImplementedError):
         LayerNorm((4, 8))
     from sparsefusion_amd.voxel_encoder import HardVFE
-    with pytest.raises(NotImplementedError, match='BatchNorm1d'):
+    with pytest.raises(NotImplementedError, match='BatchNorm'):
         HardVFE(in_channels=5, feat_channels=[64], norm_cfg=dict(type='LN'))
+    HardVFE(in_channels=5, feat_channels=[64], norm_cfg=dict(type='BN', eps=1e-3))
+
+
+def test_a_callers_own_norm_layers_keep_their_names():
+    from sparsefusion_amd.registry import NORM_LAYERS
+
+    class Own(torch.nn.LayerNorm):
+        pass
+
+    old = dict(NORM_LAYERS._modules)
+    try:
+        NORM_LAYERS._modules.pop('LN', None)
+        NORM_LAYERS.register_module('LN', module=Own)
+        for _ in range(2):
+            name, layer = build_norm_layer(dict(type='LN'), 8, postfix=1)
+            assert name == 'bn1' and type(layer) is Own
+    finally:
+        NORM_LAYERS._modules.clear()
+        NORM_LAYERS._modules.update(old)
+    assert isinstance(build_norm_layer(dict(type='LN'), 8)[1], LayerNorm)
 
 
 def test_c_entry_points_refuse_bad_arguments():
