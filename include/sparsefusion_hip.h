@@ -531,6 +531,9 @@ SF_API int sf_linear_backward(const void *dy, const void *x, long long ldx, cons
                               long long n, int dtype, int act, void *workspace,
                               size_t workspace_bytes, void *stream);
 
+/* Longest row of sf_layer_norm (column numbers, twice over, stay in 31 bits). */
+#define SF_LAYER_NORM_MOST_FEATURES (1 << 29)
+
 /* s = x + residual;  y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over rows of d elements
  * (var: the mean square, no Bessel correction).
  *   x, residual (or NULL), y, sum (s rounded, or NULL): (m, d) of dtype;  weight, bias (d) or NULL:

@@ -469,7 +469,8 @@ void dispatch(const NormArgs &a, int dtype, bool params_f32, bool backward) {
 }
 
 #define SF_NORM_CHECK_SIZES()                                                                 \
-  SF_CHECK_ARG(m >= 0 && d >= 1, "layer norm of %lld rows of %d elements", m, d);             \
+  SF_CHECK_ARG(m >= 0 && d >= 1 && d <= SF_LAYER_NORM_MOST_FEATURES,                          \
+               "layer norm of %lld rows of %d elements", m, d);                               \
   SF_CHECK_ARG(dtype >= SF_DTYPE_F32 && dtype <= SF_DTYPE_BF16, "unknown dtype %d", dtype);   \
   SF_CHECK_ARG(param_dtype == dtype || param_dtype == SF_DTYPE_F32,                           \
                "parameters must have the rows' type or be fp32 (dtype %d)", param_dtype)

@@ -14,6 +14,9 @@ from . import _lib
 from .registry import NORM_LAYERS
 
 
+MOST_FEATURES = 1 << 29      # column numbers, twice over, stay in 31 bits
+
+
 def _check(x, weight, bias):
     """-> (d, dtype code, parameters' type) of well-formed rows and parameters."""
     dtype = x.dtype
@@ -23,6 +26,8 @@ def _check(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f'layer_norm needs rows of at least one element, got {tuple(x.shape)}')
     d = x.shape[-1]
+    if d > MOST_FEATURES:
+        raise RuntimeError(f'layer_norm takes rows of up to {MOST_FEATURES} elements, got {d}')
     pdtype = None
     for name, t in (('weight', weight), ('bias', bias)):
         if t is None:

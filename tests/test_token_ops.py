@@ -158,6 +158,7 @@ def test_refusals_need_no_device():
             (lambda: linear_backward(torch.zeros(4, 6), x, w, b, activation='relu'), 'pre must have'),
             (lambda: layer_norm(x.long()), 'fp32, fp16 or bf16'),
             (lambda: layer_norm(torch.zeros(4, 0)), 'at least one element'),
+            (lambda: layer_norm(torch.zeros(1).expand((1 << 32) + 8)), 'rows of up to'),
             (lambda: layer_norm(x, torch.zeros(7)), r'shape \(8,\)'),
             (lambda: layer_norm(x, torch.zeros(8).half()), 'weight and bias'),
             (lambda: layer_norm(x.half(), torch.zeros(8), torch.zeros(8).half()), 'weight and bias'),
@@ -228,6 +229,10 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.sf_layer_norm(one, None, None, None, one, None, None, None, 4, 8, 1e-5, 1, 2, None) == -1
     assert L.sf_layer_norm(one, None, None, None, None, None, None, None, 4, 8, 1e-5, 0, 0, None) == -1
     assert L.sf_layer_norm(None, None, None, None, None, None, None, None, 0, 8, 1e-5, 0, 0, None) == 0
+    for m, d in ((4, (1 << 29) + 1), (4, -1), (-1, 8)):
+        assert L.sf_layer_norm(one, None, None, None, one, None, None, None, m, d, 1e-5, 0, 0, None) == -1
+        assert L.sf_layer_norm_backward(one, one, one, one, None, None, one, None, None, m, d, 0, 0, None,
+                                        0, None) == -1
     need = L.sf_layer_norm_backward_workspace(100, 32, 0)
     assert need >= 2 * 32 * 4
     assert L.sf_layer_norm_backward(one, one, one, one, None, None, one, one, one, 100, 32, 0, 0, one,
@@ -766,3 +771,34 @@ def test_same_inputs_same_bits_and_inputs_untouched(dev):
             assert all(torch.equal(p, q) for p, q in zip(a, linear_backward(dy, x, w, z, 'gelu')))
             assert all(torch.equal(p, q) for p, q in zip(n, layer_norm_backward(x, x, mean, rstd)))
         assert all(torch.equal(p, q) for p, q in zip(keep, (x, w, dy, z)))
+
+
+@pytest.mark.gpu
+def test_offsets_past_31_bits(dev):
+    """Tensors of more than 2^31 elements, zero but for their last rows, those against 64 bits (zero rows
+    add nothing to the sums over rows); rows far apart."""
+    m, d, dtype = 8_400_100, 256, torch.bfloat16
+    last = slice(m - 300, m)
+    x = torch.zeros(m, d, dtype=dtype, device=dev)
+    x[last] = rand(1, 300, d, dtype=dtype, dev=dev)
+    w, b = rand(2, d, dtype=dtype, dev=dev), rand(3, d, dtype=dtype, dev=dev)
+    y, _, mean, rstd = layer_norm_forward(x, w, b, keep_stats=True)
+    small = layer_norm_forward(x[last], w, b, keep_stats=True)
+    assert torch.equal(y[last], small[0]) and torch.equal(mean[last], small[2])
+    assert torch.equal(y[0], b) and torch.equal(y[m // 2], b)      # rows of zeros
+    dx, dw, db = layer_norm_backward(x, x, mean, rstd, w)      # zero gradients ahead of the last rows
+    check_norm_backward(x[last], x[last], mean[last], rstd[last], w, None, dx[last], dw, db)
+    assert not dx[:m - 300].any()
+    del y, dx
+    wl, bl = rand(4, d, d, dtype=dtype, dev=dev, scale=d ** -0.5), rand(5, d, dtype=dtype, dev=dev)
+    y, _ = linear_forward(x, wl, bl)
+    check_forward(x[last], wl, bl, None, None, y[last])
+    assert torch.equal(y[0], bl) and torch.equal(y[m // 2], bl)
+    del y
+    dx, dw, db = linear_backward(x, x, wl)
+    check_backward(x[last], x[last], wl, None, None, dx[last], dw, db)
+    assert not dx[:m - 300].any()
+    del dx
+    wide = x.view(-1)[:64 << 25].view(64, 1 << 25)[:, -64:]      # rows 2^25 elements apart
+    wide.copy_(rand(6, 64, 64, dtype=dtype, dev=dev))
+    check_forward(wide, wl[:, :64], bl, 'gelu', None, linear(wide, wl[:, :64], bl, 'gelu'))
