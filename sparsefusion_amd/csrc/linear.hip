@@ -427,8 +427,7 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   gw.out = dw;
   gx.partial = gw.partial = (float *)(base + b.split);
   if (dx && dw && b.pair) {
-    prepare(gx, b.dx);
-    prepare(gw, b.dw);
+    SF_CHECK_ARG(prepare(gx, b.dx) && prepare(gw, b.dw), "linear: %lld x %lld outputs are too many", m, k);
     rc = dtype == SF_DTYPE_F32   ? sf_gradients_f32(gx, gw, sums, st)
          : dtype == SF_DTYPE_F16 ? sf_gradients_f16(gx, gw, sums, st)
                                  : sf_gradients_bf16(gx, gw, sums, st);

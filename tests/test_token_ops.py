@@ -262,11 +262,13 @@ SIZES = [(1, 64, 64), (1, 1, 1), (3, 7, 5), (64, 64, 64), (65, 127, 63), (129, 1
          (200, 128, 256), (127, 451, 333), (257, 96, 129), (5, 8192, 40), (1, 4100, 1000),
          (1500, 200, 520), (2100, 64, 1024),
          (16, 72, 48), (17, 33, 31), (64, 1023, 65), (65, 3, 2)]
+# enough tiles for the larger shapes, whole, split and cut at the edges
+LARGE = [(4000, 512, 1024), (9000, 1024, 1000), (16300, 800, 1016), (2000, 4096, 4096)]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('m,k,n', SIZES)
+@pytest.mark.parametrize('m,k,n', SIZES + LARGE)
 def test_linear_matches_float64(dev, dtype, m, k, n):
     x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev, scale=k ** -0.5)
     b, r = rand(3, n, dtype=dtype, dev=dev), rand(4, m, n, dtype=dtype, dev=dev)
@@ -279,7 +281,7 @@ def test_linear_matches_float64(dev, dtype, m, k, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('m,k,n', SIZES + [(40000, 72, 48), (33, 300, 1111)])
+@pytest.mark.parametrize('m,k,n', SIZES + LARGE + [(40000, 72, 48), (33, 300, 1111), (40000, 64, 1024)])
 def test_linear_backward_matches_float64(dev, dtype, m, k, n):
     x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev, scale=k ** -0.5)
     dy, z = rand(3, m, n, dtype=dtype, dev=dev), rand(4, m, n, dtype=dtype, dev=dev)
@@ -418,7 +420,7 @@ def test_linear_gradients_only_where_asked_and_no_double_backward(dev):
 # ---------------------------------------------------------------------------------- layer norm
 
 NORM_SIZES = [(1, 1), (1, 64), (3, 7), (200, 128), (33, 256), (50, 333), (17, 512), (9, 1000),
-              (21, 2048), (6, 4097), (5, 8192), (3, 16384), (2, 20001), (5000, 96), (70000, 40)]
+              (21, 2048), (6, 4097), (5, 8192), (3, 16384), (2, 20001), (5000, 96), (70000, 40), (110000, 333)]
 
 
 def norm64(x, w, b, eps, r=None):
