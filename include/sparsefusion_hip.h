@@ -505,7 +505,7 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
 /* Bytes of scratch (16-byte aligned) sf_linear needs for these operands; 0 for most.  The pointers are
  * looked at, not followed: operands that are not made of aligned 16-byte pieces are copied first. */
 SF_API size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
-                                  long long k, long long n, int dtype);
+                                  long long k, long long n, int dtype, int has_residual);
 
 /* y = act(x weight^T + bias) + residual, one launch (one more when few rows meet a long k, and one for
  * operands that have to be copied).

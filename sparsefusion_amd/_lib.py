@@ -102,7 +102,7 @@ SIGNATURES = {
     'sf_dynamic_scatter_workspace': (_sz, [C.POINTER(C.c_int), _i]),
     'sf_dynamic_scatter': (_i, [_vp, _vp, _i, _i, _i, C.POINTER(C.c_int), _i, _vp, _vp, _vp, _vp,
                                 _i, _vp, _vp, _vp, _sz, _vp]),
-    'sf_linear_workspace': (_sz, [_vp, _ll, _vp, _ll, _ll, _ll, _i]),
+    'sf_linear_workspace': (_sz, [_vp, _ll, _vp, _ll, _ll, _ll, _i, _i]),
     'sf_linear': (_i, [_vp, _ll, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp, _sz, _vp]),
     'sf_linear_backward_workspace': (_sz, [_vp, _vp, _ll, _vp, _ll, _ll, _ll, _i, _i]),
     'sf_linear_backward': (_i, [_vp, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp,

@@ -466,9 +466,10 @@ __device__ __forceinline__ void sf_unroll(F &&f) {
 }
 
 // Shape of a kernel: BP x BQ outputs by WP x WQ waves, steps of STEP bytes of k in a ring of RING
-// buffers, WGS workgroups to a CU.
-template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_>
+// buffers, WGS workgroups to a CU; RES: a residual may be added.
+template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_, bool RES_ = true>
 struct SfShape {
+  static constexpr bool RES = RES_;
   static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STEP = STEP_, RING = RING_, WGS = WGS_;
   static constexpr int WAVES = WP * WQ, BYTES = (BP + BQ) * STEP, LDS = RING * BYTES + WAVES * 4096;
   static_assert(LDS * WGS <= 160 * 1024 && (RING == 2 || RING == 4), "LDS of a CU");
@@ -592,7 +593,7 @@ __device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds,
     const SfEpilogue<T, TP, TQ> epilogue{a, stage, p0, q0, split, l};
     typename SfEpilogue<T, TP, TQ>::Ahead ahead;
     const bool inside = q0 + TQ * 32 <= a.nq && p0 + TP * 32 <= a.np;
-    const bool residual = a.residual && a.splits == 1;
+    const bool residual = SH::RES && a.residual && a.splits == 1;
     // A step: the fragments of each 32 bytes of k are read while the 32 before multiply, and the
     // second half of the youngest load is issued.  Ahead of the last products the next step has landed
     // (every wave waits for its own loads, the barrier joins them) and nobody needs this step's buffer
@@ -846,7 +847,12 @@ static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
   return SF_OK;
 }
 
+// 256 x 256: steps of 128 bytes bring whole lines (those of 64 ask the L2 for each line twice), but leave no
+// registers for a residual fetched ahead.  bf16, 64 and 128 bytes: 32400 x 256 -> 1024 GELU 35.2 and
+// 33.7 us, 259200 x 1024 -> 256 167 and 160, 16384 x 2048 -> 2048 123 and 117 (1170 TFLOP/s); with a
+// residual 259200 x 1024 -> 256 takes 200 and 204, 32400 x 256 -> 1024 56 and 59.
 typedef SfShape<256, 256, 2, 4, 64, 4, 1> SfTile256;
+typedef SfShape<256, 256, 2, 4, 128, 2, 1, false> SfTile256Plain;
 typedef SfShape<128, 128, 2, 2, 128, 2, 2> SfTile128;
 // 64 x 64: deep enough to cover the latency of one workgroup alone (64 x 4096 -> 4096 bf16: 33 us with a
 // ring of 2, 21 with 4); fp32's products cover it themselves, three workgroups level the CUs better
@@ -856,13 +862,15 @@ typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64Three;
 
 template <typename T, bool PMINOR, bool QMINOR>
 static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
-  int rc;
+  int rc = SF_OK;
   if (tile == 32) {
     hipLaunchKernelGGL((sf_small_kernel<T, PMINOR, QMINOR>), dim3(a.tiles_p * a.tiles_q * a.splits), dim3(256),
                        0, st, a);
-    rc = SF_OK;
-  } else if (tile == 256) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
-  else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
+  } else if (tile == 256) {
+    if constexpr (!PMINOR && !QMINOR)      // gradients have no residual
+      if (a.residual && a.splits == 1) return sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
+    rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256Plain>(a, st);
+  } else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
   else if (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
   else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
   if (rc) return rc;

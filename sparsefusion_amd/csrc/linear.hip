@@ -15,14 +15,14 @@ struct Plan {
 // Time (us, without the launch) of t workgroups of a tile's kernel, each `per` steps of 128 bytes of k,
 // on the busiest CU; fitted to 30 sizes from 64 x 64 x 64 to 8192^3.  Two 128 x 128 tiles share a CU and
 // take hardly longer than one.
-double tile_cost(int tile, long long t, long long per, int dtype) {
+double tile_cost(int tile, long long t, long long per, int dtype, bool residual) {
   const double n = (double)((t + 255) / 256), k = (double)per;
   if (dtype == SF_DTYPE_F32)
     return tile == 256   ? n * (8 + 7.5 * k)
            : tile == 128 ? n * (2 + 2.05 * k)
            : tile == 64  ? n * (0.7 + (n < 2 ? 0.7 : 0.57) * k)
                          : n * (0.3 + 0.24 * k);
-  return tile == 256   ? n * (11 + 1.75 * k)
+  return tile == 256   ? residual ? n * (11 + 1.75 * k) : n * (7 + 1.65 * k)
          : tile == 128 ? (double)((t + 511) / 512) * (4 + k)
          : tile == 64  ? n * (0.8 + 0.3 * k)
                        : n * (0.3 + 0.165 * k);
@@ -35,7 +35,7 @@ constexpr long long kMostSmallTiles = 512;
 
 // Tile and splits of a np x nq product over nk: the cheapest of the four tiles, each whole or with the
 // contraction cut into as many parts as fill the chip.
-Plan make_plan(long long np, long long nq, long long nk, int dtype) {
+Plan make_plan(long long np, long long nq, long long nk, int dtype, bool residual) {
   const long long bk = 128 / (long long)sf_dtype_size(dtype);
   const long long steps = (nk + bk - 1) / bk;
   Plan best{128, 1, steps * bk, 1e30};
@@ -52,7 +52,7 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype) {
       const long long per = (steps + s - 1) / s;
       s = (steps + per - 1) / per;
       if (tile == 32 && t * s > kMostSmallTiles) continue;
-      double c = tile_cost(tile, t * s, per, dtype);
+      double c = tile_cost(tile, t * s, per, dtype, residual && s == 1);
       if (s > 1) c += 6 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
       if (c < best.cost) best = Plan{tile, (int)s, per * bk, c};
     }
@@ -274,12 +274,12 @@ struct BackwardPlan {
 BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const void *w, long long m,
                            long long k, long long n, int dtype, int act) {
   BackwardPlan b;
-  b.dx = make_plan(m, k, n, dtype);
-  b.dw = make_plan(n, k, m, dtype);
+  b.dx = make_plan(m, k, n, dtype, false);
+  b.dw = make_plan(n, k, m, dtype, false);
   auto small = [&](long long np, long long nq, long long nk) {
     const long long bk = 128 / (long long)sf_dtype_size(dtype), steps = (nk + bk - 1) / bk;
     const long long t = ((np + 31) / 32) * ((nq + 31) / 32);
-    return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype)};
+    return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype, false)};
   };
   // One launch for both products in 32 x 32 tiles where that is cheaper than two: a launch costs the host
   // 3 us, and one product runs in the other's idle CUs.  With one of the two gradients asked for the
@@ -307,9 +307,9 @@ struct ForwardPlan {
   size_t x, w, bytes;
 };
 ForwardPlan forward_plan(const void *x, long long ldx, const void *w, long long m, long long k, long long n,
-                         int dtype) {
+                         int dtype, bool residual) {
   ForwardPlan f;
-  f.y = make_plan(m, n, k, dtype);
+  f.y = make_plan(m, n, k, dtype, residual);
   f.pack_x = !whole_chunks(x, ldx, k, dtype);
   f.pack_w = !whole_chunks(w, k, k, dtype);
   // Few rows go without tiles (16 x 4096 -> 4096 bf16: 10.7 us against 12.1, 1 x 1024 -> 4096: 4.4 against
@@ -346,9 +346,9 @@ bool good_sizes(long long m, long long k, long long n, int dtype) {
   } while (0)
 
 extern "C" size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
-                                      long long k, long long n, int dtype) {
+                                      long long k, long long n, int dtype, int has_residual) {
   if (!good_sizes(m, k, n, dtype) || !m || !n || !k) return 0;
-  return forward_plan(x, ldx, weight, m, k, n, dtype).bytes;
+  return forward_plan(x, ldx, weight, m, k, n, dtype, has_residual != 0).bytes;
 }
 
 extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const void *bias,
@@ -364,7 +364,7 @@ extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const
   a.bias = bias, a.residual = residual, a.out = y, a.pre = pre;
   a.act = act;
   if (k == 0) return product(a, 0, dtype, Plan{128, 1, 0, 0}, st);
-  const ForwardPlan f = forward_plan(x, ldx, weight, m, k, n, dtype);
+  const ForwardPlan f = forward_plan(x, ldx, weight, m, k, n, dtype, residual != nullptr);
   if (f.few) return launch(a, 0, dtype, SF_FEW_ROWS, st);
   SF_LINEAR_CHECK_WORKSPACE("sf_linear", f.bytes);
   unsigned char *base = (unsigned char *)ws;

@@ -81,7 +81,7 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     # most sizes need no scratch: only a refusal asks how much
     rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, None, 0, stream)
     if rc == _lib.SF_ERR_WORKSPACE:
-        nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code)
+        nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code, pr is not None)
         ws = x.new_empty(nbytes, dtype=torch.uint8)
         rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, ws.data_ptr(), nbytes, stream)
     if rc:

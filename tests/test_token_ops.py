@@ -208,12 +208,12 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.sf_linear(None, 8, one, None, None, one, None, 4, 8, 4, 0, 0, None, 0, None) == -1
     assert L.sf_linear(one, 8, one, None, None, one, None, -1, 8, 4, 0, 0, None, 0, None) == -1
     assert L.sf_linear(None, 8, None, None, None, None, None, 0, 8, 4, 0, 0, None, 0, None) == 0
-    need = L.sf_linear_workspace(one, 8192, one, 80, 8192, 64, 0)      # a contraction in parts
+    need = L.sf_linear_workspace(one, 8192, one, 80, 8192, 64, 0, 0)      # a contraction in parts
     assert need > 0
     assert L.sf_linear(one, 8192, one, None, None, one, None, 80, 8192, 64, 0, 0, one, need - 1, None) == -2
     assert b'workspace' in L.sf_last_error()
-    assert L.sf_linear_workspace(one, 64, one, 80, 64, 64, 0) == 0
-    need = L.sf_linear_workspace(one + 4, 64, one, 80, 64, 64, 0)      # a copy of x
+    assert L.sf_linear_workspace(one, 64, one, 80, 64, 64, 0, 0) == 0
+    need = L.sf_linear_workspace(one + 4, 64, one, 80, 64, 64, 0, 0)      # a copy of x
     assert need >= 80 * 64 * 4
     assert L.sf_linear(one + 4, 64, one, None, None, one, None, 80, 64, 64, 0, 0, one, need - 1, None) == -2
     assert L.sf_linear(one + 4, 64, one, None, None, one, None, 80, 64, 64, 0, 0, one + 4, need, None) == -1
@@ -223,7 +223,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert need >= 64 * 32 * 2
     assert L.sf_linear_backward(one, one, 32, one, one, one, one, one, 64, 32, 32, 2, 2, one, need - 1,
                                 None) == -2
-    assert L.sf_linear_workspace(one, 4, one, -1, 4, 4, 0) == 0
+    assert L.sf_linear_workspace(one, 4, one, -1, 4, 4, 0, 0) == 0
     assert L.sf_linear_backward_workspace(one, one, 4, one, 4, 4, 4, 9, 0) == 0
     assert L.sf_layer_norm(one, None, None, None, one, None, None, None, 4, 0, 1e-5, 0, 0, None) == -1
     assert L.sf_layer_norm(one, None, None, None, one, None, None, None, 4, 8, 1e-5, 1, 2, None) == -1
