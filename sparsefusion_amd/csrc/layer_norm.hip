@@ -81,7 +81,7 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
 #pragma unroll
         for (int j = 0; j < V; ++j) v[c][j] += u[j];
       }
-      if (sum && live) sf_store_chunk<T>(sum + at, i0, d, v[c]);
+      if (sum && live) sf_store_chunk<T, NT>(sum + at, i0, d, v[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) s = fmaf(v[c][j], inv_d, s);   // zeros behind the row's end
     }
@@ -100,7 +100,7 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
     for (int c = 0; c < NV; ++c) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rs * wv[c][j] + bv[c][j];
-      sf_store_chunk<T>(y + at, (c * LANES + lane) * V, d, v[c]);
+      sf_store_chunk<T, NT>(y + at, (c * LANES + lane) * V, d, v[c]);
     }
     if (lane == 0) {
       if (mean) mean[row] = mu;
@@ -219,7 +219,7 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) u[j] += (g[c][j] - s1 - xh[c][j] * s2) * rs;
-      sf_store_chunk<T>(dx + at, i0, d, u);
+      sf_store_chunk<T, NT>(dx + at, i0, d, u);
     }
   }
   if (!part) return;
@@ -417,7 +417,7 @@ void launch_fwd(const NormArgs &a) {
   long long g = (a.m + groups - 1) / groups;
   const long long most = s.threads == 1024 ? 512 : 2048;      // every workgroup resident
   const int grid = (int)(g < most ? g : most);
-  const bool nt = (size_t)a.m * a.d * sizeof(T) >= kSfStreamBytes;
+  const bool nt = sf_streamed(a.m, (size_t)a.d * sizeof(T));
 #define SF_GO1(L, N, TH, NT)                                                                   \
   hipLaunchKernelGGL((norm_fwd_kernel<T, P, L, N, TH, NT>), dim3(grid), dim3(TH), 0, a.st,     \
                      (const T *)a.x, (const T *)a.res, a.w, a.b, (T *)a.y, (T *)a.sum, a.mean, \
@@ -442,7 +442,7 @@ void launch_bwd(const NormArgs &a) {
                          a.part, a.m, a.d);
     return;
   }
-  const bool nt = (size_t)a.m * a.d * sizeof(T) >= kSfStreamBytes;
+  const bool nt = sf_streamed(a.m, (size_t)a.d * sizeof(T));
 #define SF_GO1(L, N, TH, NT)                                                                       \
   hipLaunchKernelGGL((norm_bwd_kernel<T, P, L, N, TH, NT>), dim3(a.blocks), dim3(TH),              \
                      TH == L ? 0 : (size_t)TH * N * SfChunk<T>::V * sizeof(float), a.st,           \

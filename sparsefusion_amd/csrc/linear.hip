@@ -240,7 +240,7 @@ void run_dz(const void *dy, const void *pre, int act, void *dz, SfColumnSums &db
   const long long run = (m + want - 1) / want;
   db.part = part, db.n = n, db.runs = (int)((m + run - 1) / run);
   const dim3 grid((unsigned)((n + cl * V - 1) / (cl * V)), db.runs);
-  const bool nt = (size_t)m * n * sizeof(T) >= kSfStreamBytes;
+  const bool nt = sf_streamed(m, (size_t)n * sizeof(T));      // dz itself is read again at once
   auto kern = cl == 8    ? nt ? dz_kernel<T, 8, true> : dz_kernel<T, 8, false>
               : cl == 16 ? nt ? dz_kernel<T, 16, true> : dz_kernel<T, 16, false>
                          : nt ? dz_kernel<T, 32, true> : dz_kernel<T, 32, false>;

@@ -34,7 +34,7 @@ __device__ __forceinline__ void sf_load_chunk(const T *__restrict__ p, long long
   }
 }
 
-template <typename T>
+template <typename T, bool NT = false>
 __device__ __forceinline__ void sf_store_chunk(T *__restrict__ p, long long i0, long long n,
                                                const float *v) {
   constexpr int V = SfChunk<T>::V;
@@ -42,7 +42,9 @@ __device__ __forceinline__ void sf_store_chunk(T *__restrict__ p, long long i0, 
     typename SfChunk<T>::type c;
 #pragma unroll
     for (int j = 0; j < V; ++j) c[j] = (T)v[j];
-    *reinterpret_cast<typename SfChunk<T>::type *>(p + i0) = c;
+    auto *at = reinterpret_cast<typename SfChunk<T>::type *>(p + i0);
+    if constexpr (NT) __builtin_nontemporal_store(c, at);
+    else *at = c;
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -50,9 +52,13 @@ __device__ __forceinline__ void sf_store_chunk(T *__restrict__ p, long long i0, 
   }
 }
 
-// Streams of at least this size are read with NT loads (the last-level cache holds 256 MB, a pass has
-// four such).  Add and norm of 259200 x 256 bf16 (133 MB each): 103.7 us without, 87.4 with; its
-// gradients 104.7 and 99.6; of 5003 x 333 fp32 (7 MB each, cached): 9.2 and 10.3, gradients 15.1 and 17.3.
-constexpr size_t kSfStreamBytes = (size_t)64 << 20;
-
 static inline size_t sf_dtype_size(int dtype) { return dtype == SF_DTYPE_F32 ? 4 : 2; }
+
+// Whether m rows of `row_bytes` go around the caches, NT: tensors of 64 MB (the last-level cache holds
+// 256 MB, a pass has four such) whose rows are whole lines.  Without and with, no output written twice
+// to the same place: add and norm of 259200 x 256 bf16 104 and 98 us, of 60000 x 512 fp32 100 and 94, its
+// gradients 95 and 86; with rows that share lines (110000 x 333 fp32) 161 and 167, of cached tensors
+// (5003 x 333 fp32) 9.2 and 10.3.
+static inline bool sf_streamed(long long m, size_t row_bytes) {
+  return row_bytes % 128 == 0 && (size_t)m * row_bytes >= ((size_t)64 << 20);
+}

@@ -420,7 +420,7 @@ def test_linear_gradients_only_where_asked_and_no_double_backward(dev):
 # ---------------------------------------------------------------------------------- layer norm
 
 NORM_SIZES = [(1, 1), (1, 64), (3, 7), (200, 128), (33, 256), (50, 333), (17, 512), (9, 1000),
-              (21, 2048), (6, 4097), (5, 8192), (3, 16384), (2, 20001), (5000, 96), (70000, 40), (110000, 333)]
+              (21, 2048), (6, 4097), (5, 8192), (3, 16384), (2, 20001), (5000, 96), (70000, 40), (110000, 333), (70000, 512)]
 
 
 def norm64(x, w, b, eps, r=None):
