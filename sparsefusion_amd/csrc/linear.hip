@@ -13,17 +13,17 @@ struct Plan {
 };
 
 // Time (us, without the launch) of t workgroups of a tile's kernel, each `per` steps of 128 bytes of k,
-// on the busiest CU; fitted to 30 sizes from 64 x 64 x 64 to 8192^3.  Two 128 x 128 tiles share a CU and
-// take hardly longer than one.
+// on the busiest CU; fitted to 40 sizes from 64 x 64 x 64 to 8192^3.  Two 16-bit 128 x 128 tiles share a
+// CU and take 1.3 times as long as one alone; a 256 x 256 tile reads its residual with nothing under it.
 double tile_cost(int tile, long long t, long long per, int dtype, bool residual) {
   const double n = (double)((t + 255) / 256), k = (double)per;
   if (dtype == SF_DTYPE_F32)
-    return tile == 256   ? n * (8 + 7.5 * k)
+    return tile == 256   ? n * ((residual ? 34 : 8) + 7.5 * k)
            : tile == 128 ? n * (2 + 2.05 * k)
            : tile == 64  ? n * (0.7 + (n < 2 ? 0.7 : 0.57) * k)
                          : n * (0.3 + 0.24 * k);
-  return tile == 256   ? residual ? n * (11 + 1.75 * k) : n * (7 + 1.65 * k)
-         : tile == 128 ? (double)((t + 511) / 512) * (4 + k)
+  return tile == 256   ? residual ? n * (11 + 1.75 * k) : n * (8 + 1.65 * k)
+         : tile == 128 ? ((double)(t / 512) + (t % 512 == 0 ? 0 : t % 512 > 256 ? 1 : 0.75)) * (4 + k)
          : tile == 64  ? n * (0.8 + 0.3 * k)
                        : n * (0.3 + 0.165 * k);
 }
