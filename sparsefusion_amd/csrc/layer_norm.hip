@@ -228,9 +228,12 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
+      for (int j = 0; j < V; j += 4) {
         const int i = (c * LANES + lane) * V + j;
-        if (i < d) out[i] = aw[c][j], out[d + i] = ab[c][j];
+        if (i < d) {
+          sf_store_chunk<float>(out, i, d, &aw[c][j]);
+          sf_store_chunk<float>(out + d, i, d, &ab[c][j]);
+        }
       }
   } else {
     constexpr int W = LANES * NV * V;
