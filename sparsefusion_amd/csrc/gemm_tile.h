@@ -16,6 +16,11 @@
 // Q is the instruction's first operand, so a lane ends up with four consecutive q of one row p.
 // Workgroups stay and walk the tiles: the loads of the next tile's first steps run under the epilogue of
 // the last.
+//
+// What bounds it: a 256 x 256 tile's products of 128 bytes of k keep the matrix units busy for as long as
+// LDS takes to write the chunks and read the fragments; half of both is reached (16384 x 2048 -> 2048
+// bf16 1170 TFLOP/s; fp32 8192 x 2048 -> 2048 142 TFLOP/s, 90 % of the peak).  Short contractions are bound by the epilogue, long outputs by memory:
+// 259200 x 1024 -> 256 bf16 with its residual moves 797 MB in 193 us.
 // Rows and k outside the operands read as zeros (the buffer descriptor's range check), columns
 // outside are never stored.
 //

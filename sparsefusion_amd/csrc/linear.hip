@@ -160,7 +160,8 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
 // ---- dz and the bias gradient -------------------------------------------------------------------
 // A workgroup owns CL chunks of columns (32, fewer for narrow layers) and a run of rows, 256 / CL at a
 // time; dz goes out as it is computed, the column sums stay in registers, join through LDS and leave as
-// part[run][n].  The sums are of the fp32 products, not of the rounded dz.
+// part[run][n].  The sums are of the fp32 products, not of the rounded dz.  Bound by memory:
+// 32400 x 2048 bf16 with GELU 95 us, 398 MB.
 template <typename T, int CL, bool NT>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
