@@ -524,8 +524,8 @@ SF_API size_t sf_linear_backward_workspace(const void *dy, const void *x, long l
 /* Gradients of sf_linear for the gradient dy (m, n) of y:
  *   dz = dy act'(pre);  dx (m, k) = dz weight;  dw (n, k) = dz^T x;  db (n) = sum of dz's rows.
  * dx, dw and db may each be NULL (not wanted).  pre is not read when act is SF_ACT_NONE.  The
- * residual's gradient is dy itself.  dz is held in dtype between the passes (the products take it as
- * an operand); db sums it unrounded. */
+ * residual's gradient is dy itself.  dz is rounded to dtype (the products take it as an operand); db sums
+ * it unrounded. */
 SF_API int sf_linear_backward(const void *dy, const void *x, long long ldx, const void *weight,
                               const void *pre, void *dx, void *dw, void *db, long long m, long long k,
                               long long n, int dtype, int act, void *workspace,

@@ -74,12 +74,12 @@ __device__ __forceinline__ float sf_act(float z, int act) {
   return z;
 }
 template <typename T>
-__device__ __forceinline__ float sf_act_slope(float z, int act) {
-  if (act == SF_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float sf_act_gradient(float g, float z, int act) {
+  if (act == SF_ACT_RELU) return z <= 0.0f ? 0.0f : g;      // whatever g is
   if (act == SF_ACT_GELU)      // Phi(z) + z phi(z)
-    return fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f),
-                sf_phi<T>(z));
-  return 1.0f;
+    return g * fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f),
+                    sf_phi<T>(z));
+  return g;
 }
 
 struct SfGemmArgs {
@@ -721,6 +721,18 @@ int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnS
 int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 
+// A tiny layer's gradients without a pass ahead; dx, dw or db may be NULL.  whole: rows of all tensors are
+// whole chunks.
+struct SfGradients {
+  const void *dy, *pre, *x, *w;
+  void *dx, *dw, *db;
+  long long ldx, m, k, n;
+  int act;
+};
+int sf_tiny_gradients_f32(const SfGradients &g, bool whole, hipStream_t st);
+int sf_tiny_gradients_f16(const SfGradients &g, bool whole, hipStream_t st);
+int sf_tiny_gradients_bf16(const SfGradients &g, bool whole, hipStream_t st);
+
 // ---- small products -------------------------------------------------------------------------------
 // Too few 64 x 64 tiles to fill the chip leave each CU with one workgroup that walks a long contraction
 // alone.  Here a workgroup owns 32 x 32 outputs and its four waves share each step's 128 bytes of k, 32
@@ -731,6 +743,30 @@ int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumn
 struct SfSmall {
   static constexpr int B = 32, STEP = 128, RING = 8, BYTES = 2 * B * STEP, LDS = RING * BYTES;
 };
+
+// The sum of the four waves' blocks (in 16 KB of LDS that nobody uses any more): four columns of a row
+// for each thread, row threadIdx.x / 8, columns from 4 (threadIdx.x % 8) on.
+__device__ __forceinline__ void sf_add_shares(const sf_f32x16 &acc, unsigned char *lds, float *v) {
+  // lane (row = lane % 32, h = lane / 32) holds columns 8 g + 4 h + 0..3: the waves' blocks behind each
+  // other, quads swizzled by the row
+  float *part = reinterpret_cast<float *>(lds);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<sf_f32x4 *>(part + wave * 1024 + row * 32 + (((2 * g + h) ^ row ^ (row >> 3)) & 7) * 4) =
+        (sf_f32x4){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+  __syncthreads();
+  const int r = threadIdx.x >> 3, quad = threadIdx.x & 7;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const sf_f32x4 f =
+        *reinterpret_cast<const sf_f32x4 *>(part + w * 1024 + r * 32 + ((quad ^ r ^ (r >> 3)) & 7) * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += f[j];
+  }
+}
 
 template <typename T, bool PMINOR, bool QMINOR>
 __device__ __forceinline__ void sf_small(const SfGemmArgs &a, unsigned char *lds, int group) {
@@ -786,24 +822,9 @@ __device__ __forceinline__ void sf_small(const SfGemmArgs &a, unsigned char *lds
   }
   sf_wait_loads<0>();
   __syncthreads();
-  // lane (row = lane % 32, h = lane / 32) holds columns 8 g + 4 h + 0..3: the waves' blocks behind each
-  // other, quads swizzled by the row
-  float *part = reinterpret_cast<float *>(lds);
-  const int row = lane & 31, h = lane >> 5;
-#pragma unroll
-  for (int g = 0; g < 4; ++g)
-    *reinterpret_cast<sf_f32x4 *>(part + wave * 1024 + row * 32 + (((2 * g + h) ^ row ^ (row >> 3)) & 7) * 4) =
-        (sf_f32x4){acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
-  __syncthreads();
+  float v[4];
+  sf_add_shares(acc, lds, v);
   const int r = threadIdx.x >> 3, quad = threadIdx.x & 7;      // 32 rows by 8 quads
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const sf_f32x4 f =
-        *reinterpret_cast<const sf_f32x4 *>(part + w * 1024 + r * 32 + ((quad ^ r ^ (r >> 3)) & 7) * 4);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += f[j];
-  }
   const long long prow = p0 + r, col = q0 + 4 * quad;
   if (prow < a.np) {
     const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
@@ -937,6 +958,170 @@ static int sf_gradients_go(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfC
   return SF_OK;
 }
 
+// ---- a tiny layer's gradients in one launch, straight from dy ---------------------------------------
+// Chunk of row `row` (of n) at element i0 (of nk), zeros outside.
+template <typename T>
+__device__ __forceinline__ typename SfMfma<T>::frag sf_row_chunk(const T *p, long long ld, long long row,
+                                                                 long long n, long long i0, long long nk) {
+  constexpr int V = 16 / sizeof(T);
+  typename SfMfma<T>::frag e = {};
+  if (row < n) {
+    const T *at = p + row * ld + i0;
+    if (i0 + V <= nk) {
+      e = __builtin_bit_cast(typename SfMfma<T>::frag, *reinterpret_cast<const sf_u32x4_any *>(at));
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i0 + j < nk) e[j] = at[j];
+    }
+  }
+  return e;
+}
+
+// The 32 x 32 outputs of which four waves hold a share each: added up and stored.
+template <typename T>
+__device__ __forceinline__ void sf_store_shared(const sf_f32x16 &acc, unsigned char *lds, T *out, long long p0,
+                                                long long np, long long q0, long long nq) {
+  float v[4];
+  sf_add_shares(acc, lds, v);
+  const long long row = p0 + (threadIdx.x >> 3), col = q0 + 4 * (threadIdx.x & 7);
+  if (row >= np) return;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (col + j < nq) out[row * nq + col + j] = (T)v[j];
+}
+
+// dx = dz w, dw = dz^T x and db = sum dz of a tiny layer by different workgroups of one launch, the
+// longest first.  dz = dy act'(pre) is made where it is used, on the way from registers into LDS, so there
+// is no pass ahead and nothing to copy: loads need no alignment, and what is outside reads as zeros.
+// 32 x 32 tiles, a step's 128 bytes of k shared by the four waves, DEEP steps' loads in flight.  Bound by
+// the step: 0.4 us in fp32, in GELU's slope 0.5 (16 bits 0.7), one wave a SIMD.  400 x 256 -> 128 fp32 ReLU
+// 8.2 us, 200 x 256 -> 256 bf16 GELU 5.4; with a pass for dz ahead 9.5 and 9.7, and a launch more.
+template <typename T, bool DW, bool WHOLE>
+__device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned char *lds, int group) {
+  constexpr int B = 32, STEP = 128, V = 16 / sizeof(T), BK = STEP / (int)sizeof(T), DEEP = 4;
+  typedef SfOperand<T, DW, B, 4, STEP> OP;
+  typedef SfOperand<T, true, B, 4, STEP> OQ;
+  typedef typename SfMfma<T>::frag frag;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T *dy = static_cast<const T *>(g.dy), *pre = static_cast<const T *>(g.pre);
+  const T *q = static_cast<const T *>(DW ? g.x : g.w);
+  const long long np = DW ? g.n : g.m, nk = DW ? g.m : g.n, ldq = DW ? g.ldx : g.k;
+  const int tiles_q = (int)((g.k + B - 1) / B), steps = (int)((nk + BK - 1) / BK);
+  const long long p0 = (long long)(group / tiles_q) * B, q0 = (long long)(group % tiles_q) * B;
+  // this thread's chunk of a step of each operand: its place in LDS is 16 threadIdx.x
+  const int prow = wave * OP::RPI + lane / OP::CPR, pc = ((lane % OP::CPR) ^ OP::swz(prow)) * V;
+  const int qrow = wave * OQ::RPI + lane / OQ::CPR, qc = ((lane % OQ::CPR) ^ OQ::swz(qrow)) * V;
+  frag ry[DEEP], rz[DEEP], rq[DEEP];
+  // chunk (row0 + r, col0 + c) of a tensor of rows x cols, row0 and col0 the same for the workgroup
+  auto fetch = [&](const T *t, long long ld, long long rows, long long cols, long long row0, int r,
+                   long long col0, int c) -> frag {
+    if constexpr (WHOLE) {      // no branches: the buffer's range check makes the zeros
+      const long long left = ((rows - 1) * ld + cols - row0 * ld - col0) * (long long)sizeof(T);
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T *>(t + row0 * ld + col0), 0,
+          row0 >= rows || left < 0 ? 0 : left < 0x7FFFFFFF ? (int)left : 0x7FFFFFFF, 0x00020000);
+      const unsigned off = (unsigned)((r * ld + c) * (long long)sizeof(T));
+      return __builtin_bit_cast(frag, __builtin_amdgcn_raw_buffer_load_b128(rs, col0 + c < cols ? off : 0x80000000u, 0, 0));
+    } else {
+      return sf_row_chunk<T>(t, ld, row0 + r, col0 + c < cols ? rows : 0, col0 + c, cols);
+    }
+  };
+  auto load = [&](auto slot, int step) {
+    constexpr int D = decltype(slot)::value;
+    const long long k0 = (long long)step * BK, row0 = DW ? k0 : p0, col0 = DW ? p0 : k0;
+    ry[D] = fetch(dy, g.n, g.m, g.n, row0, prow, col0, pc);
+    if (g.act != SF_ACT_NONE) rz[D] = fetch(pre, g.n, g.m, g.n, row0, prow, col0, pc);
+    rq[D] = fetch(q, ldq, nk, g.k, k0, qrow, q0, qc);
+  };
+  auto put = [&](auto slot, unsigned char *buf) {
+    constexpr int D = decltype(slot)::value;
+    frag e = ry[D];
+    if (g.act == SF_ACT_GELU) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = (T)sf_act_gradient<T>((float)e[j], (float)rz[D][j], SF_ACT_GELU);
+    } else if (g.act == SF_ACT_RELU) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) e[j] = (T)sf_act_gradient<T>((float)e[j], (float)rz[D][j], SF_ACT_RELU);
+    }
+    *reinterpret_cast<frag *>(buf + 16 * threadIdx.x) = e;
+    *reinterpret_cast<frag *>(buf + B * STEP + 16 * threadIdx.x) = rq[D];
+  };
+  sf_f32x16 acc;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+  sf_unroll<0, DEEP>([&](auto d) { load(d, decltype(d)::value); });
+  for (int i0 = 0; i0 < steps; i0 += DEEP)
+    sf_unroll<0, DEEP>([&](auto d) {
+      const int i = i0 + decltype(d)::value;
+      if (i >= steps) return;
+      unsigned char *buf = lds + (decltype(d)::value & 1) * (2 * B * STEP);      // DEEP is even
+      put(d, buf);
+      load(d, i + DEEP);
+      // LDS only: the loads stay in flight.  The buffer of step i - 1 is free behind this barrier
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const frag fp = OP::fragment(buf, 0, wave, lane);
+      const frag fq = OQ::fragment(buf + B * STEP, 0, wave, lane);
+      acc = SfMfma<T>::run(fq, fp, acc);
+    });
+  __syncthreads();
+  sf_store_shared<T>(acc, lds, static_cast<T *>(DW ? g.dw : g.dx), p0, np, q0, g.k);
+}
+
+// db of 32 columns: the sums of the fp32 products, not of the rounded dz.
+template <typename T>
+__device__ __forceinline__ void sf_tiny_db(const SfGradients &g, float *red, int group) {
+  constexpr int V = 16 / sizeof(T), CL = 32 / V, RL = 256 / CL, DEEP = 4;
+  typedef typename SfMfma<T>::frag frag;
+  const T *dy = static_cast<const T *>(g.dy), *pre = static_cast<const T *>(g.pre);
+  const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
+  const long long col = (long long)group * 32 + cl * V;
+  float sum[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = 0.0f;
+  for (long long r = rl; r < g.m; r += RL * DEEP) {
+    frag e[DEEP], z[DEEP];
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      e[i] = sf_row_chunk<T>(dy, g.n, r + i * RL, col < g.n ? g.m : 0, col, g.n);
+      if (g.act != SF_ACT_NONE) z[i] = sf_row_chunk<T>(pre, g.n, r + i * RL, col < g.n ? g.m : 0, col, g.n);
+    }
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        sum[j] += g.act != SF_ACT_NONE ? sf_act_gradient<T>((float)e[i][j], (float)z[i][j], g.act) : (float)e[i][j];
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j) red[rl * 33 + cl * V + j] = sum[j];
+  __syncthreads();
+  if (threadIdx.x < 32 && group * 32 + threadIdx.x < g.n) {
+    float t = 0.0f;
+    for (int i = 0; i < RL; ++i) t += red[i * 33 + threadIdx.x];
+    static_cast<T *>(g.db)[group * 32 + threadIdx.x] = (T)t;
+  }
+}
+
+template <typename T, bool WHOLE>
+__global__ void __launch_bounds__(256) sf_tiny_gradients_kernel(SfGradients g, int dw_groups, int dx_groups) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 32 * 128];
+  const int b = blockIdx.x;
+  if (b < dw_groups) sf_tiny_gradient<T, true, WHOLE>(g, lds, b);
+  else if (b < dw_groups + dx_groups) sf_tiny_gradient<T, false, WHOLE>(g, lds, b - dw_groups);
+  else sf_tiny_db<T>(g, reinterpret_cast<float *>(lds), b - dw_groups - dx_groups);
+}
+
+template <typename T>
+static int sf_tiny_gradients_go(const SfGradients &g, bool whole, hipStream_t st) {
+  const long long tq = (g.k + 31) / 32;
+  const int nw = g.dw ? (int)((g.n + 31) / 32 * tq) : 0, nx = g.dx ? (int)((g.m + 31) / 32 * tq) : 0;
+  const int nb = g.db ? (int)((g.n + 31) / 32) : 0;
+  if (!(nw + nx + nb)) return SF_OK;
+  auto kern = whole ? sf_tiny_gradients_kernel<T, true> : sf_tiny_gradients_kernel<T, false>;
+  hipLaunchKernelGGL(kern, dim3(nw + nx + nb), dim3(256), 0, st, g, nw, nx);
+  return SF_OK;
+}
+
 // ---- few rows -------------------------------------------------------------------------------------
 // y of few rows: bound by the weight's bytes and by latency, so there is no tile in LDS
 // and no pipeline.  A workgroup owns 16 columns and 16 TP rows; its 8 waves share the contraction in
@@ -963,25 +1148,6 @@ template <> struct SfMfma16<__bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
 };
-
-// Chunk of row `row` (of n) at element i0 (of nk), zeros outside.
-template <typename T>
-__device__ __forceinline__ typename SfMfma<T>::frag sf_row_chunk(const T *p, long long ld, long long row,
-                                                                 long long n, long long i0, long long nk) {
-  constexpr int V = 16 / sizeof(T);
-  typename SfMfma<T>::frag e = {};
-  if (row < n) {
-    const T *at = p + row * ld + i0;
-    if (i0 + V <= nk) {
-      e = __builtin_bit_cast(typename SfMfma<T>::frag, *reinterpret_cast<const sf_u32x4_any *>(at));
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (i0 + j < nk) e[j] = at[j];
-    }
-  }
-  return e;
-}
 
 template <typename T, int TP>
 __global__ void __launch_bounds__(512) sf_few_rows_kernel(SfGemmArgs a) {

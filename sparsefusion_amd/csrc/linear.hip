@@ -189,7 +189,7 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
         if (r + RL * i >= r1) break;
         if (act != SF_ACT_NONE) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] *= sf_act_slope<T>(z[i][j], act);
+          for (int j = 0; j < V; ++j) g[i][j] = sf_act_gradient<T>(g[i][j], z[i][j], act);
         }
         // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a
         // ReLU's or GELU's gradient of zero is zero
@@ -268,6 +268,7 @@ int zero_out(void *p, long long elements, int dtype, hipStream_t st) {
 // Where the pieces of the backward pass's workspace start, and what is copied first.
 struct BackwardPlan {
   Plan dx, dw;
+  bool tiny;      // everything in one launch and without workspace
   bool pair;      // both products in one launch
   bool write_dz, pack_x, pack_w;
   size_t dz, x, w, part, split, bytes;
@@ -282,11 +283,28 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
     const long long t = ((np + 31) / 32) * ((nq + 31) / 32);
     return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype, false)};
   };
-  // One launch for both products in 32 x 32 tiles where that is cheaper than two: a launch costs the host
-  // 3 us, and one product runs in the other's idle CUs.  With one of the two gradients asked for the
-  // tiles stay the same, so that its values do.
+  // Three ways, by cost (us, each launch 3): dz (and db's parts) by a pass of its own, then the two products
+  // in one launch each; or both in one launch of 32 x 32 tiles, the one in the other's idle CUs; or these
+  // tiles alone, making dz as they read dy.  That is work for each tile again (us a step below), worth it
+  // while the steps are few: 400 x 256 -> 128 fp32 ReLU 8.2 us (pass and pair 9.5), bf16 GELU 7.9 (10.1),
+  // 500 x 512 -> 512 bf16 ReLU 9.4 (11.8), GELU 14.2 (12.5), 1000 x 512 -> 512 fp32 GELU 35 (25).  With one
+  // of the gradients asked for the tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
+  const double pass = act == SF_ACT_NONE ? 5 : 6.5;
+  const double two = pass + 9 + b.dx.cost + b.dw.cost, pair = pass + 0.8 * (x32.cost + w32.cost);
   b.pair = k > 0 && m < (1 << 20) && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
+  const long long bk = 128 / (long long)sf_dtype_size(dtype), tq = (k + 31) / 32;
+  const double sx = (double)((n + bk - 1) / bk), sw = (double)((m + bk - 1) / bk);
+  const double work = ((double)((m + 31) / 32 * tq) * sx + (double)((n + 31) / 32 * tq) * sw) / 256;
+  const double longest = sx > sw ? sx : sw;
+  const double step = dtype == SF_DTYPE_F32 ? act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
+                                            : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
+  const double tiny = 3 + step * (work > longest ? work : longest);
+  b.tiny = k > 0 && work < 1000 && longest < 1000 && tiny < (b.pair ? pair : two);
+  if (b.tiny) {
+    b.bytes = 0;
+    return b;
+  }
   if (b.pair) b.dx = x32, b.dw = w32;
   b.write_dz = act != SF_ACT_NONE || !whole_chunks(dy, n, n, dtype);
   b.pack_x = !whole_chunks(x, ldx, k, dtype);
@@ -401,6 +419,16 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   SF_CHECK_ARG(dy && (pre || act == SF_ACT_NONE) && (weight || !dx) && (x || !dw), "NULL tensor pointer");
   const BackwardPlan b = backward_plan(dy, x, ldx, weight, m, k, n, dtype, act);
   SF_LINEAR_CHECK_WORKSPACE("sf_linear_backward", b.bytes);
+  if (b.tiny) {
+    const SfGradients g{dy, pre, x, weight, dx, dw, db, ldx, m, k, n, act};
+    const bool whole = whole_chunks(dy, n, n, dtype) && whole_chunks(pre, n, n, dtype) &&
+                       whole_chunks(x, ldx, k, dtype) && whole_chunks(weight, k, k, dtype);
+    rc = dtype == SF_DTYPE_F32   ? sf_tiny_gradients_f32(g, whole, st)
+         : dtype == SF_DTYPE_F16 ? sf_tiny_gradients_f16(g, whole, st)
+                                 : sf_tiny_gradients_bf16(g, whole, st);
+    SF_CHECK_LAUNCH();
+    return rc;
+  }
   unsigned char *base = (unsigned char *)ws;
   const void *dz = dy;
   long long ldz = n;

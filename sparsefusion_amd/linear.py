@@ -118,13 +118,14 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     db = x.new_empty(n) if needs[2] else None
     L = _lib.lib()
     pg, px, pw = grad.data_ptr(), rows.data_ptr(), weight.data_ptr()
-    nbytes = L.sf_linear_backward_workspace(pg, px, ldx, pw, m, k, n, code, act)
-    ws = _lib.workspace(nbytes, x)
-    rc = L.sf_linear_backward(
-        pg, px, ldx, pw,
-        None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
-        None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code,
-        act, None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
+    args = (pg, px, ldx, pw, None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
+            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code, act)
+    stream = _lib.stream(x.device)
+    rc = L.sf_linear_backward(*args, None, 0, stream)      # tiny layers need no scratch
+    if rc == _lib.SF_ERR_WORKSPACE:
+        nbytes = L.sf_linear_backward_workspace(pg, px, ldx, pw, m, k, n, code, act)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
+        rc = L.sf_linear_backward(*args, ws.data_ptr(), nbytes, stream)
     if rc:
         _lib.check(rc)
     return dx, dw, db

@@ -219,9 +219,9 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.sf_linear(one + 4, 64, one, None, None, one, None, 80, 64, 64, 0, 0, one + 4, need, None) == -1
     assert b'aligned' in L.sf_last_error()
     assert L.sf_linear_backward(one, one, 8, one, None, one, one, one, 4, 8, 4, 0, 2, None, 0, None) == -1
-    need = L.sf_linear_backward_workspace(one, one, 32, one, 64, 32, 32, 2, 2)
-    assert need >= 64 * 32 * 2
-    assert L.sf_linear_backward(one, one, 32, one, one, one, one, one, 64, 32, 32, 2, 2, one, need - 1,
+    need = L.sf_linear_backward_workspace(one, one, 32, one, 6400, 32, 32, 2, 2)
+    assert need >= 6400 * 32 * 2
+    assert L.sf_linear_backward(one, one, 32, one, one, one, one, one, 6400, 32, 32, 2, 2, one, need - 1,
                                 None) == -2
     assert L.sf_linear_workspace(one, 4, one, -1, 4, 4, 0, 0) == 0
     assert L.sf_linear_backward_workspace(one, one, 4, one, 4, 4, 4, 9, 0) == 0
@@ -360,6 +360,15 @@ def test_linear_infinities_and_nan_stay_in_their_rows(dev, dtype):
     assert (y[3] == float('inf')).all() and y[77].isnan().all() and (y[129] == -float('inf')).all()
     act = linear(x2, w, activation='relu')
     assert (act[3] == float('inf')).all() and act[77].isnan().all() and not act[129].any()
+    # what ReLU blocks stays blocked, whatever it is
+    for m in (130, 9000):
+        x, z = rand(3, m, 64, dtype=dtype, dev=dev), rand(4, m, 70, dtype=dtype, dev=dev)
+        dy = rand(5, m, 70, dtype=dtype, dev=dev)
+        masked = dy.masked_fill(z <= 0, 0)
+        dy[z <= 0] = torch.tensor([float('inf'), float('nan'), -float('inf')], dtype=dtype,
+                                  device=dev).repeat(m * 70)[:int((z <= 0).sum())]
+        got, want = linear_backward(dy, x, w, z, 'relu'), linear_backward(masked, x, w, z, 'relu')
+        assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
 
 
 @pytest.mark.gpu
