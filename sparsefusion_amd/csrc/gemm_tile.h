@@ -1123,11 +1123,10 @@ static int sf_tiny_gradients_go(const SfGradients &g, bool whole, hipStream_t st
 }
 
 // ---- few rows -------------------------------------------------------------------------------------
-// y of few rows: bound by the weight's bytes and by latency, so there is no tile in LDS
-// and no pipeline.  A workgroup owns 16 columns and 16 TP rows; its 8 waves share the contraction in
-// turns of 64 bytes of k and each loads its operands' fragments straight from memory, all in flight
-// at once (lane = row % 16, 16-byte chunk lane / 16: a row's 64 bytes are one line's half).  The waves'
-// sums meet in LDS and each wave finishes its share of the outputs.
+// y of up to 16 rows: bound by the weight's bytes and by latency, so there is no tile in LDS and no
+// pipeline.  A workgroup owns 16 columns; its 8 waves share the contraction in turns of 4 x 64 bytes of k
+// and each loads its operands' fragments straight from memory, all in flight at once (lane = row % 16,
+// 16-byte chunk lane / 16: a row's 64 bytes are one line's half).  The waves' sums meet in LDS.
 template <typename T> struct SfMfma16;
 template <> struct SfMfma16<float> {
   static __device__ __forceinline__ sf_f32x4 run(SfMfma<float>::frag a, SfMfma<float>::frag b, sf_f32x4 c) {
@@ -1149,52 +1148,43 @@ template <> struct SfMfma16<__bf16> {
   }
 };
 
-template <typename T, int TP>
+template <typename T>
 __global__ void __launch_bounds__(512) sf_few_rows_kernel(SfGemmArgs a) {
   constexpr int V = 16 / sizeof(T), WAVES = 8, UNROLL = 4;
-  __shared__ float part[WAVES][TP][64][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
-  const long long q0 = (long long)(blockIdx.x % a.tiles_q) * 16, p0 = (long long)(blockIdx.x / a.tiles_q) * 16 * TP;
+  __shared__ float part[WAVES][64][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, c = lane >> 4;
+  const long long q0 = (long long)blockIdx.x * 16;
   const T *p = static_cast<const T *>(a.p), *q = static_cast<const T *>(a.q);
-  sf_f32x4 acc[TP];
-#pragma unroll
-  for (int t = 0; t < TP; ++t) acc[t] = (sf_f32x4){0.f, 0.f, 0.f, 0.f};
-  constexpr int K = 4 * V;      // k of a turn
+  sf_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  constexpr int K = 4 * V;      // k of 64 bytes
   for (long long k0 = wave * K; k0 < a.nk; k0 += UNROLL * WAVES * K) {
-    typename SfMfma<T>::frag fq[UNROLL], fp[UNROLL][TP];
+    typename SfMfma<T>::frag fq[UNROLL], fp[UNROLL];
 #pragma unroll
     for (int i = 0; i < UNROLL; ++i) {
       const long long k = k0 + i * WAVES * K + c * V;
-      fq[i] = sf_row_chunk<T>(q, a.ldq, q0 + r, k < a.nk ? a.nq : 0, k, a.nk);
-#pragma unroll
-      for (int t = 0; t < TP; ++t)
-        fp[i][t] = sf_row_chunk<T>(p, a.ldp, p0 + 16 * t + r, k < a.nk ? a.np : 0, k, a.nk);
+      fq[i] = sf_row_chunk<T>(q, a.ldq, q0 + row, k < a.nk ? a.nq : 0, k, a.nk);
+      fp[i] = sf_row_chunk<T>(p, a.ldp, row, k < a.nk ? a.np : 0, k, a.nk);
     }
 #pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-#pragma unroll
-      for (int t = 0; t < TP; ++t) acc[t] = SfMfma16<T>::run(fq[i], fp[i][t], acc[t]);
+    for (int i = 0; i < UNROLL; ++i) acc = SfMfma16<T>::run(fq[i], fp[i], acc);
   }
   // accumulator: row p = lane % 16, columns q = 4 (lane / 16) + 0..3
-#pragma unroll
-  for (int t = 0; t < TP; ++t) *reinterpret_cast<sf_f32x4 *>(part[wave][t][lane]) = acc[t];
+  *reinterpret_cast<sf_f32x4 *>(part[wave][lane]) = acc;
   __syncthreads();
-  if (threadIdx.x >= TP * 64) return;
-  const int t = threadIdx.x >> 6;
+  if (wave) return;
   float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int w = 0; w < WAVES; ++w)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += part[w][t][lane][j];
-  const long long row = p0 + 16 * t + r, col = q0 + 4 * c;
+    for (int j = 0; j < 4; ++j) v[j] += part[w][lane][j];
   if (row >= a.np) return;
   const T *bias = static_cast<const T *>(a.bias), *res = static_cast<const T *>(a.residual);
   T *out = static_cast<T *>(a.out), *pre = static_cast<T *>(a.pre);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (col + j >= a.nq) break;
-    const long long at = row * a.nq + col + j;
-    float z = v[j] + (bias ? (float)bias[col + j] : 0.0f);
+    const long long col = q0 + 4 * c + j, at = row * a.nq + col;
+    if (col >= a.nq) break;
+    float z = v[j] + (bias ? (float)bias[col] : 0.0f);
     if (pre) pre[at] = (T)z;
     z = sf_act<T>(z, a.act);
     out[at] = (T)(z + (res ? (float)res[at] : 0.0f));
@@ -1202,13 +1192,8 @@ __global__ void __launch_bounds__(512) sf_few_rows_kernel(SfGemmArgs a) {
 }
 
 template <typename T>
-static int sf_few_rows(SfGemmArgs a, hipStream_t st) {
-  const int tp = a.np <= 16 ? 1 : a.np <= 32 ? 2 : 4;
-  a.tiles_q = (int)((a.nq + 15) / 16);
-  const dim3 grid((unsigned)(a.tiles_q * ((a.np + 16 * tp - 1) / (16 * tp))));
-  if (tp == 1) hipLaunchKernelGGL((sf_few_rows_kernel<T, 1>), grid, dim3(512), 0, st, a);
-  else if (tp == 2) hipLaunchKernelGGL((sf_few_rows_kernel<T, 2>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((sf_few_rows_kernel<T, 4>), grid, dim3(512), 0, st, a);
+static int sf_few_rows(const SfGemmArgs &a, hipStream_t st) {
+  hipLaunchKernelGGL((sf_few_rows_kernel<T>), dim3((unsigned)((a.nq + 15) / 16)), dim3(512), 0, st, a);
   return SF_OK;
 }
 

@@ -53,7 +53,7 @@ Plan make_plan(long long np, long long nq, long long nk, int dtype, bool residua
       s = (steps + per - 1) / per;
       if (tile == 32 && t * s > kMostSmallTiles) continue;
       double c = tile_cost(tile, t * s, per, dtype, residual && s == 1);
-      if (s > 1) c += 6 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
+      if (s > 1) c += 4.5 + 8e-6 * (double)(np * nq * s) / 4.5;      // the parts' round trip and a launch
       if (c < best.cost) best = Plan{tile, (int)s, per * bk, c};
     }
   }
@@ -319,6 +319,20 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   return b;
 }
 
+// Whether up to 16 rows go without tiles, by the turns a wave takes at k (us each) and the weight's bytes.
+// In us, without and with tiles: 1 x 1024 -> 4096 bf16 4.2 and 6.1, 4096 -> 4096 10.0 and 13.3; the turns
+// of a long k for few columns are better spread over workgroups (fp32 4096 -> 64 14 and 6.3), and 16-bit
+// rows that start anywhere take long turns (4095 -> 65 bf16 17 and 10, the copy included).
+bool few_rows(long long m, long long k, long long n, int dtype, bool copy, double tiles) {
+  const double bytes = (double)n * k * sf_dtype_size(dtype), memory = bytes / 4.9e6;
+  const double turn = dtype == SF_DTYPE_F32 ? (m > 4 ? 1.8 : 1.4)
+                      : copy                ? (m > 4 ? 6 : 3.6)
+                                            : (m > 4 ? 1.7 : 1.1);
+  const double turns = turn * (double)k * sf_dtype_size(dtype) / 2048;
+  if (copy) tiles += 4 + 2 * memory;
+  return 1.8 + (turns > memory ? turns : memory) < 2.7 + (tiles > memory ? tiles : memory);
+}
+
 // The same for the forward pass.
 struct ForwardPlan {
   Plan y;
@@ -331,10 +345,7 @@ ForwardPlan forward_plan(const void *x, long long ldx, const void *w, long long 
   f.y = make_plan(m, n, k, dtype, residual);
   f.pack_x = !whole_chunks(x, ldx, k, dtype);
   f.pack_w = !whole_chunks(w, k, k, dtype);
-  // Few rows go without tiles (16 x 4096 -> 4096 bf16: 10.7 us against 12.1, 1 x 1024 -> 4096: 4.4 against
-  // 8.2, 64 x 4096 -> 4096: 22 against 12.8), more of them where the tiles would need a copy
-  // (64 x 1023 -> 1023 bf16: 21 us).
-  f.few = m <= 16 || (m <= 64 && (f.pack_x || f.pack_w));
+  f.few = m <= 16 && few_rows(m, k, n, dtype, f.pack_x || f.pack_w, f.y.cost);
   if (f.few) f.y.splits = 1, f.pack_x = f.pack_w = false;
   f.x = align256(partial_bytes(f.y, m, n));
   f.w = f.x + (f.pack_x ? padded_bytes(m, k, dtype) : 0);
