@@ -5,10 +5,11 @@
 //   dw = sum_rows dy xh;  db = sum_rows dy
 //
 // Both directions are bound by memory: every tensor is read or written once, the row lives in
-// registers between its loads and its stores (the variance is the centred second pass over those
-// registers, so a large common offset costs no digits; the mean is summed from s / d, so rows whose sum
-// passes fp32's range keep theirs), and all sums are fp32.  259200 x 256 bf16, 531 MB each way: add and
-// norm 97 us (5.5 TB/s), gradients 95 us and 5 for the join; a copy of that size moves 4.9 TB/s.
+// registers between its loads (all in flight at once) and its stores (the variance is the centred second
+// pass over those registers, so a large common offset costs no digits; the mean is summed from s / d, so
+// rows whose sum passes fp32's range keep theirs), and all sums are fp32.  259200 x 256 bf16, 531 MB each
+// way: add and norm 92 us (5.8 TB/s), gradients 91 us and 5 for the join; a copy of that size moves
+// 4.9 TB/s.
 //
 // A row belongs to a group of LANES lanes, each holding NV 16-byte chunks of it: 8 to 64 lanes of a
 // wave for short rows, so that no lane idles at 128 channels, up to a whole workgroup of 1024 lanes
@@ -51,7 +52,7 @@ __device__ __forceinline__ void load_param(const void *p, int i0, int n, float f
   for (int j = 0; j < V; ++j) v[j] = (q && i0 + j < n) ? (float)q[i0 + j] : fallback;
 }
 
-template <typename T, typename P, int LANES, int NV, int THREADS, bool NT>
+template <typename T, typename P, int LANES, int NV, int THREADS, int MODE>
 __global__ void __launch_bounds__(THREADS)
 norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *w, const void *b,
                 T *__restrict__ y, T *__restrict__ sum, float *__restrict__ mean,
@@ -72,17 +73,21 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
     const long long at = (live ? row : 0) * d;
     float v[NV][V];
     float s = 0.0f;
+    typename SfChunk<T>::type rx[NV], rr[NV];      // the row's loads, all in flight
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
-      const int i0 = (c * LANES + lane) * V;
-      sf_load_chunk<T, NT>(x + at, i0, d, v[c]);
-      if (res) {
-        float u[V];
-        sf_load_chunk<T, NT>(res + at, i0, d, u);
+      rx[c] = sf_load_raw<T, MODE>(x + at, (c * LANES + lane) * V, d);
+      if (res) rr[c] = sf_load_raw<T, MODE>(res + at, (c * LANES + lane) * V, d);
+    }
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[c][j] += u[j];
+    for (int c = 0; c < NV; ++c) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = (float)rx[c][j];
+      if (res) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[c][j] += (float)rr[c][j];
       }
-      if (sum && live) sf_store_chunk<T, NT>(sum + at, i0, d, v[c]);
+      if (sum && live) sf_store_chunk<T, MODE == SF_STREAM>(sum + at, (c * LANES + lane) * V, d, v[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) s = fmaf(v[c][j], inv_d, s);   // zeros behind the row's end
     }
@@ -101,7 +106,7 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
     for (int c = 0; c < NV; ++c) {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rs * wv[c][j] + bv[c][j];
-      sf_store_chunk<T, NT>(y + at, (c * LANES + lane) * V, d, v[c]);
+      sf_store_chunk<T, MODE == SF_STREAM>(y + at, (c * LANES + lane) * V, d, v[c]);
     }
     if (lane == 0) {
       if (mean) mean[row] = mu;
@@ -162,7 +167,7 @@ norm_fwd_long_kernel(const T *__restrict__ x, const T *__restrict__ res, const v
 }
 
 // dx of every row and, in part[block][2][d] (fp32), the workgroup's share of dw and db.
-template <typename T, typename P, int LANES, int NV, int THREADS, bool NT>
+template <typename T, typename P, int LANES, int NV, int THREADS, int MODE>
 __global__ void __launch_bounds__(THREADS)
 norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *__restrict__ mean,
                 const float *__restrict__ rstd, const void *w, const T *__restrict__ dsum,
@@ -186,13 +191,20 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
     const float mu = mean[live ? row : 0], rs = rstd[live ? row : 0];
     float g[NV][V], xh[NV][V];
     float s1 = 0.0f, s2 = 0.0f;
+    typename SfChunk<T>::type ry[NV], rx[NV], rd[NV];      // the row's loads, all in flight
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      ry[c] = sf_load_raw<T, MODE>(dy + at, (c * LANES + lane) * V, d);
+      rx[c] = sf_load_raw<T, MODE>(x + at, (c * LANES + lane) * V, d);
+      if (dsum) rd[c] = sf_load_raw<T, MODE>(dsum + at, (c * LANES + lane) * V, d);
+    }
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
       const int i0 = (c * LANES + lane) * V;
-      sf_load_chunk<T, NT>(dy + at, i0, d, g[c]);
-      sf_load_chunk<T, NT>(x + at, i0, d, xh[c]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
+        g[c][j] = (float)ry[c][j];
+        xh[c][j] = (float)rx[c][j];
         // g is zero behind the row's end, so xh there (a product of nothing but the mean) is harmless
         // unless it is not finite: it is cleared as well
         xh[c][j] = i0 + j < d ? (xh[c][j] - mu) * rs : 0.0f;
@@ -212,15 +224,12 @@ norm_bwd_kernel(const T *__restrict__ dy, const T *__restrict__ x, const float *
     for (int c = 0; c < NV; ++c) {
       const int i0 = (c * LANES + lane) * V;
       float u[V];
-      if (dsum) {
-        sf_load_chunk<T, NT>(dsum + at, i0, d, u);
-      } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) u[j] = 0.0f;
+      for (int j = 0; j < V; ++j) {
+        u[j] = (g[c][j] - s1 - xh[c][j] * s2) * rs;
+        if (dsum) u[j] += (float)rd[c][j];
       }
-#pragma unroll
-      for (int j = 0; j < V; ++j) u[j] += (g[c][j] - s1 - xh[c][j] * s2) * rs;
-      sf_store_chunk<T, NT>(dx + at, i0, d, u);
+      sf_store_chunk<T, MODE == SF_STREAM>(dx + at, i0, d, u);
     }
   }
   if (!part) return;
@@ -383,13 +392,21 @@ long long chunk_count(int d, int dtype) {
   return ((long long)d + v - 1) / v;
 }
 
-// Workgroups of the backward pass: enough to fill the chip (8 resident a CU), few enough that the
-// partial sums stay small beside the rows.
+// Most workgroups of a kernel: a CU with more of them in flight than it needs moves less (259200 x 256
+// bf16, gradients of 1024, 768 and 512 workgroups 98, 93 and 102 us, add and norm 93, 93 and 109, of 2048
+// 105; 40000 x 1024 bf16 gradients 72, 65 and 62); rows that share lines want one more a CU (110000 x 333
+// fp32 124 and 139 us of 1024 and 768).
+long long most_blocks(const NormShape &s, int d, int dtype) {
+  if (s.threads == 1024) return 256;
+  return d % (int)(16 / sf_dtype_size(dtype)) ? 1024 : 768;
+}
+
+// Workgroups of the backward pass.
 int bwd_blocks(long long m, int d, int dtype) {
   const NormShape s = norm_shape(chunk_count(d, dtype));
   const int groups = s.lanes ? s.threads / s.lanes : 1;
   long long b = (m + groups - 1) / groups;
-  const long long most = s.threads == 1024 ? 512 : 1024;
+  const long long most = s.lanes ? most_blocks(s, d, dtype) : 512;
   if (s.lanes == 0) b = (m + 63) / 64;      // norm_cols_long_kernel: 64 rows or more each
   return (int)(b < 1 ? 1 : b > most ? most : b);
 }
@@ -419,14 +436,17 @@ void launch_fwd(const NormArgs &a) {
   }
   const int groups = s.threads / s.lanes;
   long long g = (a.m + groups - 1) / groups;
-  const long long most = s.threads == 1024 ? 512 : 2048;      // every workgroup resident
+  const long long most = most_blocks(s, a.d, sizeof(T) == 4 ? SF_DTYPE_F32 : SF_DTYPE_F16);
   const int grid = (int)(g < most ? g : most);
-  const bool nt = sf_streamed(a.m, (size_t)a.d * sizeof(T));
-#define SF_GO1(L, N, TH, NT)                                                                   \
-  hipLaunchKernelGGL((norm_fwd_kernel<T, P, L, N, TH, NT>), dim3(grid), dim3(TH), 0, a.st,     \
+  const int mode = a.d % SfChunk<T>::V ? SF_RAGGED : sf_streamed(a.m, (size_t)a.d * sizeof(T)) ? SF_STREAM : SF_WHOLE;
+#define SF_GO1(L, N, TH, MODE)                                                                 \
+  hipLaunchKernelGGL((norm_fwd_kernel<T, P, L, N, TH, MODE>), dim3(grid), dim3(TH), 0, a.st,     \
                      (const T *)a.x, (const T *)a.res, a.w, a.b, (T *)a.y, (T *)a.sum, a.mean, \
                      a.rstd, a.m, a.d, a.eps)
-#define SF_GO(L, N, TH) if (nt && TH == 256) SF_GO1(L, N, TH, (TH == 256)); else SF_GO1(L, N, TH, false)
+#define SF_GO(L, N, TH)                                   \
+  if (mode == SF_RAGGED) SF_GO1(L, N, TH, SF_RAGGED);     \
+  else if (mode == SF_WHOLE) SF_GO1(L, N, TH, SF_WHOLE);  \
+  else SF_GO1(L, N, TH, SF_STREAM)
   SF_NORM_SHAPES(SF_GO);
 #undef SF_GO
 #undef SF_GO1
@@ -446,13 +466,16 @@ void launch_bwd(const NormArgs &a) {
                          a.part, a.m, a.d);
     return;
   }
-  const bool nt = sf_streamed(a.m, (size_t)a.d * sizeof(T));
-#define SF_GO1(L, N, TH, NT)                                                                       \
-  hipLaunchKernelGGL((norm_bwd_kernel<T, P, L, N, TH, NT>), dim3(a.blocks), dim3(TH),              \
+  const int mode = a.d % SfChunk<T>::V ? SF_RAGGED : sf_streamed(a.m, (size_t)a.d * sizeof(T)) ? SF_STREAM : SF_WHOLE;
+#define SF_GO1(L, N, TH, MODE)                                                                     \
+  hipLaunchKernelGGL((norm_bwd_kernel<T, P, L, N, TH, MODE>), dim3(a.blocks), dim3(TH),              \
                      TH == L ? 0 : (size_t)TH * N * SfChunk<T>::V * sizeof(float), a.st,           \
                      (const T *)a.dy, (const T *)a.x, a.mean, a.rstd, a.w, (const T *)a.sum,       \
                      (T *)a.y, a.part, a.m, a.d)
-#define SF_GO(L, N, TH) if (nt && TH == 256) SF_GO1(L, N, TH, (TH == 256)); else SF_GO1(L, N, TH, false)
+#define SF_GO(L, N, TH)                                   \
+  if (mode == SF_RAGGED) SF_GO1(L, N, TH, SF_RAGGED);     \
+  else if (mode == SF_WHOLE) SF_GO1(L, N, TH, SF_WHOLE);  \
+  else SF_GO1(L, N, TH, SF_STREAM)
   SF_NORM_SHAPES(SF_GO);
 #undef SF_GO
 #undef SF_GO1

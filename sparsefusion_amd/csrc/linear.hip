@@ -161,12 +161,13 @@ int product(SfGemmArgs &a, int layout, int dtype, const Plan &pl, hipStream_t st
 // A workgroup owns CL chunks of columns (32, fewer for narrow layers) and a run of rows, 256 / CL at a
 // time; dz goes out as it is computed, the column sums stay in registers, join through LDS and leave as
 // part[run][n].  The sums are of the fp32 products, not of the rounded dz.  Bound by memory:
-// 32400 x 2048 bf16 with GELU 95 us, 398 MB.
-template <typename T, int CL, bool NT>
+// 32400 x 2048 bf16 with GELU 75 us, 398 MB at 5.3 TB/s (four rows in flight instead of two 73, ragged and
+// fp32 rows slower; converting where they are loaded, one at a time, 87).
+template <typename T, int CL, int MODE>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__restrict__ dz, long long ldz,
           float *__restrict__ part, long long m, long long n, long long run) {
-  constexpr int V = 16 / sizeof(T), DEEP = 4, RL = 256 / CL;
+  constexpr int V = 16 / sizeof(T), DEEP = 2, RL = 256 / CL;
   __shared__ float red[RL][CL * V + 4];
   const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
   const long long col = ((long long)blockIdx.x * CL + cl) * V;
@@ -177,25 +178,28 @@ dz_kernel(const T *__restrict__ dy, const T *__restrict__ pre, int act, T *__res
   if (col < n)
     for (long long r = r0 + rl; r < r1; r += RL * DEEP) {
       // DEEP rows' loads in flight; rows past the run are read again and count for nothing
-      float g[DEEP][V], z[DEEP][V];
+      typename SfChunk<T>::type gr[DEEP], zr[DEEP];
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
         const long long row = r + RL * i < r1 ? r + RL * i : r;
-        sf_load_chunk<T, NT>(dy + row * n, col, n, g[i]);
-        if (act != SF_ACT_NONE) sf_load_chunk<T, NT>(pre + row * n, col, n, z[i]);
+        gr[i] = sf_load_raw<T, MODE>(dy + row * n, (int)col, (int)n);
+        if (act != SF_ACT_NONE) zr[i] = sf_load_raw<T, MODE>(pre + row * n, (int)col, (int)n);
       }
 #pragma unroll
       for (int i = 0; i < DEEP; ++i) {
         if (r + RL * i >= r1) break;
+        float g[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) g[j] = (float)gr[i][j];
         if (act != SF_ACT_NONE) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) g[i][j] = sf_act_gradient<T>(g[i][j], z[i][j], act);
+          for (int j = 0; j < V; ++j) g[j] = sf_act_gradient<T>(g[j], (float)zr[i][j], act);
         }
         // rows of dz are whole chunks; behind the n-th column dy and pre were read as zeros, and a
         // ReLU's or GELU's gradient of zero is zero
-        if (dz) sf_store_chunk<T>(dz + (r + RL * i) * ldz, col, ldz, g[i]);
+        if (dz) sf_store_chunk<T>(dz + (r + RL * i) * ldz, col, ldz, g);
 #pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] += g[i][j];
+        for (int j = 0; j < V; ++j) sum[j] += g[j];
       }
     }
   if (!part) return;
@@ -219,7 +223,7 @@ __global__ void __launch_bounds__(32 * TY) db_join_kernel(SfColumnSums c) {
 }
 
 // Chunks of columns to a workgroup of dz_kernel, and its runs of rows: about 2048 workgroups in all, at
-// least four turns of rows each.  (259200 x 64 bf16: 29 us with 8 chunks, 66 with 32.)
+// least four turns of rows each.  (259200 x 64 bf16: 19 us with 8 chunks, 66 with 32.)
 int dz_chunks(long long n, int dtype) {
   const long long v = 16 / (long long)sf_dtype_size(dtype), chunks = (n + v - 1) / v;
   return chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
@@ -241,10 +245,14 @@ void run_dz(const void *dy, const void *pre, int act, void *dz, SfColumnSums &db
   const long long run = (m + want - 1) / want;
   db.part = part, db.n = n, db.runs = (int)((m + run - 1) / run);
   const dim3 grid((unsigned)((n + cl * V - 1) / (cl * V)), db.runs);
-  const bool nt = sf_streamed(m, (size_t)n * sizeof(T));      // dz itself is read again at once
-  auto kern = cl == 8    ? nt ? dz_kernel<T, 8, true> : dz_kernel<T, 8, false>
-              : cl == 16 ? nt ? dz_kernel<T, 16, true> : dz_kernel<T, 16, false>
-                         : nt ? dz_kernel<T, 32, true> : dz_kernel<T, 32, false>;
+  // dz itself is read again at once
+  const int mode = n % V ? SF_RAGGED : sf_streamed(m, (size_t)n * sizeof(T)) ? SF_STREAM : SF_WHOLE;
+  auto pick = [&](auto ragged, auto whole, auto stream) {
+    return mode == SF_RAGGED ? ragged : mode == SF_WHOLE ? whole : stream;
+  };
+  auto kern = cl == 8    ? pick(dz_kernel<T, 8, SF_RAGGED>, dz_kernel<T, 8, SF_WHOLE>, dz_kernel<T, 8, SF_STREAM>)
+              : cl == 16 ? pick(dz_kernel<T, 16, SF_RAGGED>, dz_kernel<T, 16, SF_WHOLE>, dz_kernel<T, 16, SF_STREAM>)
+                         : pick(dz_kernel<T, 32, SF_RAGGED>, dz_kernel<T, 32, SF_WHOLE>, dz_kernel<T, 32, SF_STREAM>);
   hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, (const T *)dy, (const T *)pre, act, (T *)dz,
                      padded(n, dtype), db.out ? part : nullptr, m, n, run);
 }

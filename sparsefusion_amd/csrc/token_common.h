@@ -15,17 +15,13 @@ struct SfChunk {
   typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-// V values at p + i0 of a row of n elements as fp32; zeros behind its end.  NT: a load that leaves the
-// caches to others, for tensors that do not fit them anyway.
-template <typename T, bool NT = false>
+// V values at p + i0 of a row of n elements as fp32; zeros behind its end.
+template <typename T>
 __device__ __forceinline__ void sf_load_chunk(const T *__restrict__ p, long long i0, long long n,
                                               float *v) {
   constexpr int V = SfChunk<T>::V;
   if (i0 + V <= n) {
-    const auto *at = reinterpret_cast<const typename SfChunk<T>::type *>(p + i0);
-    typename SfChunk<T>::type c;
-    if constexpr (NT) c = __builtin_nontemporal_load(at);
-    else c = *at;
+    const typename SfChunk<T>::type c = *reinterpret_cast<const typename SfChunk<T>::type *>(p + i0);
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = (float)c[j];
   } else {
@@ -54,11 +50,35 @@ __device__ __forceinline__ void sf_store_chunk(T *__restrict__ p, long long i0, 
 
 static inline size_t sf_dtype_size(int dtype) { return dtype == SF_DTYPE_F32 ? 4 : 2; }
 
+// How a kernel's rows lie: RAGGED, some chunk is cut by the row's end; WHOLE, none is; STREAM, none is and
+// they go around the caches.
+enum { SF_RAGGED, SF_WHOLE, SF_STREAM };
+
+// V values at p + i0 of a row of n elements as they are, zeros behind its end.  Nothing waits for them
+// here: converting inside the branch would, a load at a time.
+template <typename T, int MODE>
+__device__ __forceinline__ typename SfChunk<T>::type sf_load_raw(const T *__restrict__ p, int i0, int n) {
+  constexpr int V = SfChunk<T>::V;
+  typename SfChunk<T>::type c;
+#pragma unroll
+  for (int j = 0; j < V; ++j) c[j] = (T)0.0f;
+  if (MODE == SF_RAGGED ? i0 + V <= n : i0 < n) {
+    const auto *at = reinterpret_cast<const typename SfChunk<T>::type *>(p + i0);
+    if constexpr (MODE == SF_STREAM) c = __builtin_nontemporal_load(at);
+    else c = *at;
+  } else if (MODE == SF_RAGGED && i0 < n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (i0 + j < n) c[j] = p[i0 + j];
+  }
+  return c;
+}
+
 // Whether m rows of `row_bytes` go around the caches, NT: tensors of 64 MB (the last-level cache holds
 // 256 MB, a pass has four such) whose rows are whole lines.  Without and with, no output written twice
 // to the same place: add and norm of 259200 x 256 bf16 104 and 98 us, of 60000 x 512 fp32 100 and 94, its
 // gradients 95 and 86; with rows that share lines (110000 x 333 fp32) 161 and 167, of cached tensors
-// (5003 x 333 fp32) 9.2 and 10.3.
+// (5003 x 333 fp32) 9.2 and 10.3.  (Measured before the row's loads went out together.)
 static inline bool sf_streamed(long long m, size_t row_bytes) {
   return row_bytes % 128 == 0 && (size_t)m * row_bytes >= ((size_t)64 << 20);
 }
