@@ -298,15 +298,18 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   // 500 x 512 -> 512 bf16 ReLU 9.4 (11.8), GELU 14.2 (12.5), 1000 x 512 -> 512 fp32 GELU 35 (25).  With one
   // of the gradients asked for the tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
-  const double pass = act == SF_ACT_NONE ? 5 : 6.5;
+  const bool whole = whole_chunks(dy, n, n, dtype) && whole_chunks(x, ldx, k, dtype) &&
+                     whole_chunks(w, k, k, dtype);
+  const double pass = (act == SF_ACT_NONE ? 5 : 6.5) + (whole ? 0 : 4);      // odd operands are copied first
   const double two = pass + 9 + b.dx.cost + b.dw.cost, pair = pass + 0.8 * (x32.cost + w32.cost);
   b.pair = k > 0 && m < (1 << 20) && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
   const long long bk = 128 / (long long)sf_dtype_size(dtype), tq = (k + 31) / 32;
   const double sx = (double)((n + bk - 1) / bk), sw = (double)((m + bk - 1) / bk);
   const double work = ((double)((m + 31) / 32 * tq) * sx + (double)((n + 31) / 32 * tq) * sw) / 256;
   const double longest = sx > sw ? sx : sw;
-  const double step = dtype == SF_DTYPE_F32 ? act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
-                                            : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
+  const double step = dtype == SF_DTYPE_F32
+                          ? !whole ? 0.85 : act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
+                          : !whole ? 1.4 : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
   const double tiny = 3 + step * (work > longest ? work : longest);
   b.tiny = k > 0 && work < 1000 && longest < 1000 && tiny < (b.pair ? pair : two);
   if (b.tiny) {
