@@ -490,7 +490,7 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
  * the LiDAR map are made of.  Storage is fp32, fp16 or bf16; all sums are fp32 and a value is rounded
  * once, when it is stored.  Nothing here uses atomics: the same inputs give the same bits.  Rows are
  * contiguous unless a row distance is an argument; no pointer needs more than its element's alignment
- * (16-byte aligned rows of a multiple of 16 bytes are faster).  Outputs must not overlap inputs. */
+ * (rows that start at multiples of 4 bytes are faster, of 16 fastest).  Outputs must not overlap inputs. */
 #define SF_DTYPE_F32 0
 #define SF_DTYPE_F16 1
 #define SF_DTYPE_BF16 2
@@ -503,7 +503,7 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
 #define SF_LINEAR_MOST_FEATURES (1 << 20)
 
 /* Bytes of scratch (16-byte aligned) sf_linear needs for these operands; 0 for most.  The pointers are
- * looked at, not followed: operands that are not made of aligned 16-byte pieces are copied first. */
+ * looked at, not followed: operands whose rows start at an odd number of 16-bit elements are copied first. */
 SF_API size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
                                   long long k, long long n, int dtype, int has_residual);
 

@@ -88,6 +88,7 @@ struct SfGemmArgs {
   long long np, nq, nk;           // output rows, output columns, contraction
   long long k_split;              // contraction of one split (a multiple of the k step)
   int tiles_p, tiles_q, splits;
+  int tail;                       // whether what is behind a K-major operand's rows has to be cleared
   const void *bias, *residual;    // (nq), (np, nq) of T or NULL
   void *out, *pre;                // (np, nq) of T; pre: the values before the activation, or NULL
   float *partial;                 // (splits, np, nq): the sums alone, when splits > 1
@@ -155,7 +156,7 @@ struct SfOperand {
   }
 
   const T *at;              // the step being loaded: the tile's first row / column at its k
-  long long rows;           // output rows this operand has from the tile's first on, whole chunks
+  long long rows;           // output rows this operand has from the tile's first on
   long long ld;
   int steps, last_k;        // steps to go in this tile, k of its last one
   unsigned range, range_last;       // bytes from `at` to the last element of a step in use
@@ -172,23 +173,34 @@ struct SfOperand {
       voff[j] = (unsigned)((long long)row * ld * S) + c * 16u;
     }
   }
-  // A tile: output rows `first` on (of `total`), k from k0 on in `steps` steps, the last of last_k.  The
-  // contiguous extent is made of whole chunks (the host repacks an operand whose is not, with zeros
-  // behind); rows past the range read as zeros (all of it fits 31 bits: the host sees to that too).
+  // A tile: output rows `first` on (of `total`), k from k0 on in `steps` steps, the last of last_k.  Rows
+  // start at multiples of 4 bytes; rows past the range read as zeros, a dword at a time (all of it fits 31
+  // bits: the host sees to both).  A chunk that a row's end cuts brings what is behind it: other columns'
+  // outputs, which nobody stores, or for a K-major operand k that clear() makes zeros.
   __device__ __forceinline__ void open(const void *ptr, long long first, long long total, long long k0,
                                        int steps_, int last_k_) {
     steps = steps_;
     at = static_cast<const T *>(ptr) + (KMINOR ? first + k0 * ld : first * ld + k0);
     if constexpr (KMINOR) {
-      rows = ((total + V - 1) & ~(long long)(V - 1)) - first, last_k = last_k_;
-      range = (unsigned)(((BK - 1) * ld + rows) * S);
-      range_last = (unsigned)(((last_k - 1) * ld + rows) * S);
+      rows = total - first, last_k = last_k_;
+      range = (unsigned)(((BK - 1) * ld + rows) * S + 3) & ~3u;
+      range_last = (unsigned)(((last_k - 1) * ld + rows) * S + 3) & ~3u;
     } else {
-      rows = total - first, last_k = (last_k_ + V - 1) & ~(V - 1);
+      rows = total - first, last_k = last_k_;
       const int n = rows < B ? (int)rows : B;
-      range = (unsigned)(((n - 1) * ld + BK) * S);
-      range_last = (unsigned)(((n - 1) * ld + last_k) * S);
+      range = (unsigned)(((n - 1) * ld + BK) * S + 3) & ~3u;
+      range_last = (unsigned)(((n - 1) * ld + last_k) * S + 3) & ~3u;
     }
+  }
+  // Zeros behind the first `k` of a step's rows (inside a chunk) at `tile`, by the whole workgroup.
+  static __device__ __forceinline__ void clear(unsigned char *tile, int k) {
+    if constexpr (!KMINOR)
+      for (int row = threadIdx.x; row < B; row += WAVES * 64) {
+        T *chunk = reinterpret_cast<T *>(tile + row * STEP + ((k / V ^ swz(row)) << 4));
+#pragma unroll
+        for (int j = 1; j < V; ++j)
+          if (j >= k % V) chunk[j] = (T)0.0f;
+      }
   }
   __device__ __forceinline__ void close() {      // nothing left to load: zeros from here on
     range = range_last = 0;
@@ -474,7 +486,7 @@ __device__ __forceinline__ void sf_unroll(F &&f) {
 // buffers, WGS workgroups to a CU; RES: a residual may be added.
 template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_, bool RES_ = true>
 struct SfShape {
-  static constexpr bool RES = RES_;
+  static constexpr bool RES = RES_, TAIL = BP_ < 256;      // TAIL: clears what is behind cut rows
   static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STEP = STEP_, RING = RING_, WGS = WGS_;
   static constexpr int WAVES = WP * WQ, BYTES = (BP + BQ) * STEP, LDS = RING * BYTES + WAVES * 4096;
   static_assert(LDS * WGS <= 160 * 1024 && (RING == 2 || RING == 4), "LDS of a CU");
@@ -492,6 +504,7 @@ template <typename T, bool PMINOR, bool QMINOR, typename SH>
 __device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds, int group, int groups) {
   constexpr int BP = SH::BP, BQ = SH::BQ, WQ = SH::WQ, WAVES = SH::WAVES, STEP = SH::STEP;
   constexpr int RING = SH::RING, BYTES = SH::BYTES, BK = STEP / (int)sizeof(T), NS = STEP / 32;
+  constexpr int V = 16 / sizeof(T);
   constexpr int TP = BP / SH::WP / 32, TQ = BQ / WQ / 32;
   typedef SfOperand<T, PMINOR, BP, WAVES, STEP> OP;
   typedef SfOperand<T, QMINOR, BQ, WAVES, STEP> OQ;
@@ -568,6 +581,16 @@ __device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds,
     __builtin_amdgcn_sched_barrier(0);
   };
 
+  // behind the barrier that shows step `step` of tile `t` in `buf`
+  auto clear_tail = [&](int t, int step, int buf) {
+    int tp, tq, split;
+    sf_tile_of(t, tiles, a, &tp, &tq, &split);
+    const long long left = a.nk - split * a.k_split - (long long)step * BK;
+    if (left >= BK || left % V == 0) return;
+    OP::clear(lds + buf, (int)left);
+    OQ::clear(lds + buf + BP * STEP, (int)left);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
   int cur = 0, last = (RING - 1) * BYTES;      // last: the buffer whose load is half issued
   open();
 #pragma unroll
@@ -579,6 +602,7 @@ __device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds,
   sf_wait_loads<(RING - 2) * NI + HALF>();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  if (SH::TAIL && a.tail && group < tiles) clear_tail(group, 0, 0);
   for (int tile = group; tile < tiles; tile += groups) {
     int tp, tq, split;
     sf_tile_of(tile, tiles, a, &tp, &tq, &split);
@@ -617,6 +641,10 @@ __device__ __forceinline__ void sf_gemm(const SfGemmArgs &a, unsigned char *lds,
       sf_wait_loads<(RING - 2) * NI>();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
+      if (SH::TAIL && a.tail && i + 2 >= steps) {
+        if (i + 2 == steps) clear_tail(tile, i + 1, nxt);
+        else if (tile + groups < tiles) clear_tail(tile + groups, 0, nxt);
+      }
       if (i + 1 == steps && inside && residual) epilogue.prefetch(ahead, 0);
       multiply(SfInt<1>(), nxt, 0, SfInt<0>(), SfInt<HALF>(), cur);
       last = cur;
@@ -709,8 +737,8 @@ static void sf_gemm_join(const SfGemmArgs &a, hipStream_t st) {
 }
 
 // The launches of one storage type (linear_f32.hip, linear_f16.hip, linear_bf16.hip).
-// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.  tile 32, 64, 128 or 256, operands of whole
-// aligned 16-byte chunks; layout 0 only: SF_FEW_ROWS, any operands.
+// layout 0: P, Q K-major; 1: Q K-minor; 2: both K-minor.  tile 32, 64, 128 or 256, operands whose rows
+// start at multiples of 4 bytes; layout 0 only: SF_FEW_ROWS, any operands.
 #define SF_FEW_ROWS 16
 int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
 int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st);
@@ -721,17 +749,17 @@ int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnS
 int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st);
 
-// A tiny layer's gradients without a pass ahead; dx, dw or db may be NULL.  whole: rows of all tensors are
-// whole chunks.
+// A tiny layer's gradients without a pass ahead; dx, dw or db may be NULL.  direct: rows of all tensors
+// start at multiples of 4 bytes.
 struct SfGradients {
   const void *dy, *pre, *x, *w;
   void *dx, *dw, *db;
   long long ldx, m, k, n;
   int act;
 };
-int sf_tiny_gradients_f32(const SfGradients &g, bool whole, hipStream_t st);
-int sf_tiny_gradients_f16(const SfGradients &g, bool whole, hipStream_t st);
-int sf_tiny_gradients_bf16(const SfGradients &g, bool whole, hipStream_t st);
+int sf_tiny_gradients_f32(const SfGradients &g, bool direct, hipStream_t st);
+int sf_tiny_gradients_f16(const SfGradients &g, bool direct, hipStream_t st);
+int sf_tiny_gradients_bf16(const SfGradients &g, bool direct, hipStream_t st);
 
 // ---- small products -------------------------------------------------------------------------------
 // Too few 64 x 64 tiles to fill the chip leave each CU with one workgroup that walks a long contraction
@@ -813,6 +841,11 @@ __device__ __forceinline__ void sf_small(const SfGemmArgs &a, unsigned char *lds
     sf_wait_loads<(RING - 2) * NI>();
     __builtin_amdgcn_s_barrier();      // step i has landed, everyone has read step i - 1
     asm volatile("" ::: "memory");
+    if (a.tail && i + 1 == steps && last_k % V) {
+      OP::clear(lds + cur, last_k);
+      OQ::clear(lds + cur + B * STEP, last_k);
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
     const frag fp = OP::fragment(lds + cur, 0, wave, lane);
     const frag fq = OQ::fragment(lds + cur + B * STEP, 0, wave, lane);
     load(old);
@@ -897,7 +930,7 @@ static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
       if (a.residual && a.splits == 1) return sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
     rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256Plain>(a, st);
   } else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
-  else if (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
+  else if constexpr (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
   else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
   if (rc) return rc;
   if (a.splits > 1) sf_gemm_join<T>(a, st);
@@ -997,7 +1030,7 @@ __device__ __forceinline__ void sf_store_shared(const sf_f32x16 &acc, unsigned c
 // 32 x 32 tiles, a step's 128 bytes of k shared by the four waves, DEEP steps' loads in flight.  Bound by
 // the step: 0.4 us in fp32, in GELU's slope 0.5 (16 bits 0.7), one wave a SIMD.  400 x 256 -> 128 fp32 ReLU
 // 8.2 us, 200 x 256 -> 256 bf16 GELU 5.4; with a pass for dz ahead 9.5 and 9.7, and a launch more.
-template <typename T, bool DW, bool WHOLE>
+template <typename T, bool DW, bool DIRECT>
 __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned char *lds, int group) {
   constexpr int B = 32, STEP = 128, V = 16 / sizeof(T), BK = STEP / (int)sizeof(T), DEEP = 4;
   typedef SfOperand<T, DW, B, 4, STEP> OP;
@@ -1016,11 +1049,11 @@ __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned 
   // chunk (row0 + r, col0 + c) of a tensor of rows x cols, row0 and col0 the same for the workgroup
   auto fetch = [&](const T *t, long long ld, long long rows, long long cols, long long row0, int r,
                    long long col0, int c) -> frag {
-    if constexpr (WHOLE) {      // no branches: the buffer's range check makes the zeros
+    if constexpr (DIRECT) {      // no branches: the buffer's range check makes the zeros
       const long long left = ((rows - 1) * ld + cols - row0 * ld - col0) * (long long)sizeof(T);
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<T *>(t + row0 * ld + col0), 0,
-          row0 >= rows || left < 0 ? 0 : left < 0x7FFFFFFF ? (int)left : 0x7FFFFFFF, 0x00020000);
+          row0 >= rows || left < 0 ? 0 : left < 0x7FFFFFF0 ? ((int)left + 3) & ~3 : 0x7FFFFFF0, 0x00020000);
       const unsigned off = (unsigned)((r * ld + c) * (long long)sizeof(T));
       return __builtin_bit_cast(frag, __builtin_amdgcn_raw_buffer_load_b128(rs, col0 + c < cols ? off : 0x80000000u, 0, 0));
     } else {
@@ -1034,7 +1067,7 @@ __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned 
     if (g.act != SF_ACT_NONE) rz[D] = fetch(pre, g.n, g.m, g.n, row0, prow, col0, pc);
     rq[D] = fetch(q, ldq, nk, g.k, k0, qrow, q0, qc);
   };
-  auto put = [&](auto slot, unsigned char *buf) {
+  auto put = [&](auto slot, int step, unsigned char *buf) {
     constexpr int D = decltype(slot)::value;
     frag e = ry[D];
     if (g.act == SF_ACT_GELU) {
@@ -1044,6 +1077,11 @@ __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned 
 #pragma unroll
       for (int j = 0; j < V; ++j) e[j] = (T)sf_act_gradient<T>((float)e[j], (float)rz[D][j], SF_ACT_RELU);
     }
+    if constexpr (!DW && DIRECT)
+      if (g.n % V) {      // a chunk that dy's row end cuts brings the next row's first values
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = (long long)step * BK + pc + j < g.n ? e[j] : (T)0.0f;
+      }
     *reinterpret_cast<frag *>(buf + 16 * threadIdx.x) = e;
     *reinterpret_cast<frag *>(buf + B * STEP + 16 * threadIdx.x) = rq[D];
   };
@@ -1056,7 +1094,7 @@ __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned 
       const int i = i0 + decltype(d)::value;
       if (i >= steps) return;
       unsigned char *buf = lds + (decltype(d)::value & 1) * (2 * B * STEP);      // DEEP is even
-      put(d, buf);
+      put(d, i, buf);
       load(d, i + DEEP);
       // LDS only: the loads stay in flight.  The buffer of step i - 1 is free behind this barrier
       asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -1102,22 +1140,22 @@ __device__ __forceinline__ void sf_tiny_db(const SfGradients &g, float *red, int
   }
 }
 
-template <typename T, bool WHOLE>
+template <typename T, bool DIRECT>
 __global__ void __launch_bounds__(256) sf_tiny_gradients_kernel(SfGradients g, int dw_groups, int dx_groups) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[4 * 32 * 128];
   const int b = blockIdx.x;
-  if (b < dw_groups) sf_tiny_gradient<T, true, WHOLE>(g, lds, b);
-  else if (b < dw_groups + dx_groups) sf_tiny_gradient<T, false, WHOLE>(g, lds, b - dw_groups);
+  if (b < dw_groups) sf_tiny_gradient<T, true, DIRECT>(g, lds, b);
+  else if (b < dw_groups + dx_groups) sf_tiny_gradient<T, false, DIRECT>(g, lds, b - dw_groups);
   else sf_tiny_db<T>(g, reinterpret_cast<float *>(lds), b - dw_groups - dx_groups);
 }
 
 template <typename T>
-static int sf_tiny_gradients_go(const SfGradients &g, bool whole, hipStream_t st) {
+static int sf_tiny_gradients_go(const SfGradients &g, bool direct, hipStream_t st) {
   const long long tq = (g.k + 31) / 32;
   const int nw = g.dw ? (int)((g.n + 31) / 32 * tq) : 0, nx = g.dx ? (int)((g.m + 31) / 32 * tq) : 0;
   const int nb = g.db ? (int)((g.n + 31) / 32) : 0;
   if (!(nw + nx + nb)) return SF_OK;
-  auto kern = whole ? sf_tiny_gradients_kernel<T, true> : sf_tiny_gradients_kernel<T, false>;
+  auto kern = direct ? sf_tiny_gradients_kernel<T, true> : sf_tiny_gradients_kernel<T, false>;
   hipLaunchKernelGGL(kern, dim3(nw + nx + nb), dim3(256), 0, st, g, nw, nx);
   return SF_OK;
 }

@@ -35,12 +35,13 @@ constexpr long long kMostSmallTiles = 512;
 
 // Tile and splits of a np x nq product over nk: the cheapest of the four tiles, each whole or with the
 // contraction cut into as many parts as fill the chip.
-Plan make_plan(long long np, long long nq, long long nk, int dtype, bool residual) {
+Plan make_plan(long long np, long long nq, long long nk, int dtype, bool residual, bool tail) {
   const long long bk = 128 / (long long)sf_dtype_size(dtype);
   const long long steps = (nk + bk - 1) / bk;
   Plan best{128, 1, steps * bk, 1e30};
   if (np < 1 || nq < 1 || nk < 1) return best;      // no product
   for (int tile : {256, 128, 64, 32}) {
+    if (tile == 256 && tail) continue;      // has no registers left to clear what is behind cut rows
     const long long t = ((np + tile - 1) / tile) * ((nq + tile - 1) / tile);
     for (int full = 0; full < 2; ++full) {
       const int slots = 256 * (tile == 256 ? 1 : tile == 64 ? 3 : 2);
@@ -66,13 +67,13 @@ size_t partial_bytes(const Plan &pl, long long np, long long nq) {
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // ---- operands of odd shapes -----------------------------------------------------------------------
-// The tiles load whole aligned 16-byte chunks.  An operand whose rows are not made of such is copied
-// first, rows padded with zeros to whole chunks.  (Loading them through registers was built and timed:
-// 3001 x 451 -> 333 fp16 13.4 us, 32401 x 255 -> 1023 bf16 87 us, both bound by the waits for loads that
-// cannot run ahead.)
-bool whole_chunks(const void *p, long long ld, long long extent, int dtype) {
-  const long long v = 16 / (long long)sf_dtype_size(dtype);
-  return (uintptr_t)p % 16 == 0 && ld % v == 0 && extent % v == 0 && ld <= 2 * SF_LINEAR_MOST_FEATURES;
+// The tiles load chunks from any multiple of 4 bytes.  An operand whose rows start elsewhere (an odd number
+// of 16-bit elements) is copied first, rows padded with zeros to whole chunks.  (Loading them through
+// registers was built and timed: 3001 x 451 -> 333 fp16 13.4 us, 32401 x 255 -> 1023 bf16 87 us, both bound
+// by the waits for loads that cannot run ahead.)
+bool direct(const void *p, long long ld, int dtype) {
+  return (uintptr_t)p % 4 == 0 && ld * (long long)sf_dtype_size(dtype) % 4 == 0 &&
+         ld <= 2 * SF_LINEAR_MOST_FEATURES;
 }
 long long padded(long long cols, int dtype) {
   const long long v = 16 / (long long)sf_dtype_size(dtype);
@@ -278,14 +279,16 @@ struct BackwardPlan {
   Plan dx, dw;
   bool tiny;      // everything in one launch and without workspace
   bool pair;      // both products in one launch
-  bool write_dz, pack_x, pack_w;
+  bool write_dz, pack_x, pack_w, tail;
   size_t dz, x, w, part, split, bytes;
 };
 BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const void *w, long long m,
                            long long k, long long n, int dtype, int act) {
   BackwardPlan b;
-  b.dx = make_plan(m, k, n, dtype, false);
-  b.dw = make_plan(n, k, m, dtype, false);
+  b.write_dz = act != SF_ACT_NONE || !direct(dy, n, dtype);
+  b.tail = n * (long long)sf_dtype_size(dtype) % 16 != 0 && !b.write_dz;      // a written dz has zeros there
+  b.dx = make_plan(m, k, n, dtype, false, b.tail);
+  b.dw = make_plan(n, k, m, dtype, false, false);
   auto small = [&](long long np, long long nq, long long nk) {
     const long long bk = 128 / (long long)sf_dtype_size(dtype), steps = (nk + bk - 1) / bk;
     const long long t = ((np + 31) / 32) * ((nq + 31) / 32);
@@ -298,9 +301,8 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   // 500 x 512 -> 512 bf16 ReLU 9.4 (11.8), GELU 14.2 (12.5), 1000 x 512 -> 512 fp32 GELU 35 (25).  With one
   // of the gradients asked for the tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
-  const bool whole = whole_chunks(dy, n, n, dtype) && whole_chunks(x, ldx, k, dtype) &&
-                     whole_chunks(w, k, k, dtype);
-  const double pass = (act == SF_ACT_NONE ? 5 : 6.5) + (whole ? 0 : 4);      // odd operands are copied first
+  const bool copy = !direct(x, ldx, dtype) || !direct(w, k, dtype), all = !copy && direct(dy, n, dtype);
+  const double pass = (act == SF_ACT_NONE ? 5 : 6.5) + (copy ? 4 : 0);
   const double two = pass + 9 + b.dx.cost + b.dw.cost, pair = pass + 0.8 * (x32.cost + w32.cost);
   b.pair = k > 0 && m < (1 << 20) && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
   const long long bk = 128 / (long long)sf_dtype_size(dtype), tq = (k + 31) / 32;
@@ -308,8 +310,8 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   const double work = ((double)((m + 31) / 32 * tq) * sx + (double)((n + 31) / 32 * tq) * sw) / 256;
   const double longest = sx > sw ? sx : sw;
   const double step = dtype == SF_DTYPE_F32
-                          ? !whole ? 0.85 : act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
-                          : !whole ? 1.4 : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
+                          ? !all ? 0.85 : act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
+                          : !all ? 1.4 : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
   const double tiny = 3 + step * (work > longest ? work : longest);
   b.tiny = k > 0 && work < 1000 && longest < 1000 && tiny < (b.pair ? pair : two);
   if (b.tiny) {
@@ -317,9 +319,8 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
     return b;
   }
   if (b.pair) b.dx = x32, b.dw = w32;
-  b.write_dz = act != SF_ACT_NONE || !whole_chunks(dy, n, n, dtype);
-  b.pack_x = !whole_chunks(x, ldx, k, dtype);
-  b.pack_w = !whole_chunks(w, k, k, dtype);
+  b.pack_x = !direct(x, ldx, dtype);
+  b.pack_w = !direct(w, k, dtype);
   b.dz = 0;
   b.x = b.write_dz ? padded_bytes(m, n, dtype) : 0;
   b.w = b.x + (b.pack_x ? padded_bytes(m, k, dtype) : 0);
@@ -347,15 +348,16 @@ bool few_rows(long long m, long long k, long long n, int dtype, bool copy, doubl
 // The same for the forward pass.
 struct ForwardPlan {
   Plan y;
-  bool few, pack_x, pack_w;
+  bool few, pack_x, pack_w, tail;
   size_t x, w, bytes;
 };
 ForwardPlan forward_plan(const void *x, long long ldx, const void *w, long long m, long long k, long long n,
                          int dtype, bool residual) {
   ForwardPlan f;
-  f.y = make_plan(m, n, k, dtype, residual);
-  f.pack_x = !whole_chunks(x, ldx, k, dtype);
-  f.pack_w = !whole_chunks(w, k, k, dtype);
+  f.pack_x = !direct(x, ldx, dtype);
+  f.pack_w = !direct(w, k, dtype);
+  f.tail = k * (long long)sf_dtype_size(dtype) % 16 != 0 && !(f.pack_x && f.pack_w);
+  f.y = make_plan(m, n, k, dtype, residual, f.tail);
   f.few = m <= 16 && few_rows(m, k, n, dtype, f.pack_x || f.pack_w, f.y.cost);
   if (f.few) f.y.splits = 1, f.pack_x = f.pack_w = false;
   f.x = align256(partial_bytes(f.y, m, n));
@@ -414,6 +416,7 @@ extern "C" int sf_linear(const void *x, long long ldx, const void *weight, const
   const Repack pw{f.pack_w ? weight : nullptr, base + f.w, k, n, k};
   const int rc = repack(px, pw, dtype, st);
   if (rc) return rc;
+  a.tail = f.tail;
   if (f.pack_x) a.p = px.dst, a.ldp = padded(k, dtype);
   if (f.pack_w) a.q = pw.dst, a.ldq = padded(k, dtype);
   return product(a, 0, dtype, f.y, st);
@@ -443,11 +446,11 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   SF_LINEAR_CHECK_WORKSPACE("sf_linear_backward", b.bytes);
   if (b.tiny) {
     const SfGradients g{dy, pre, x, weight, dx, dw, db, ldx, m, k, n, act};
-    const bool whole = whole_chunks(dy, n, n, dtype) && whole_chunks(pre, n, n, dtype) &&
-                       whole_chunks(x, ldx, k, dtype) && whole_chunks(weight, k, k, dtype);
-    rc = dtype == SF_DTYPE_F32   ? sf_tiny_gradients_f32(g, whole, st)
-         : dtype == SF_DTYPE_F16 ? sf_tiny_gradients_f16(g, whole, st)
-                                 : sf_tiny_gradients_bf16(g, whole, st);
+    const bool all = direct(dy, n, dtype) && direct(pre, n, dtype) && direct(x, ldx, dtype) &&
+                     direct(weight, k, dtype);
+    rc = dtype == SF_DTYPE_F32   ? sf_tiny_gradients_f32(g, all, st)
+         : dtype == SF_DTYPE_F16 ? sf_tiny_gradients_f16(g, all, st)
+                                 : sf_tiny_gradients_bf16(g, all, st);
     SF_CHECK_LAUNCH();
     return rc;
   }
@@ -473,6 +476,7 @@ extern "C" int sf_linear_backward(const void *dy, const void *x, long long ldx, 
   gx.p = dz, gx.q = pw.src ? pw.dst : weight, gx.ldp = ldz, gx.ldq = pw.src ? padded(k, dtype) : k;
   gx.np = m, gx.nq = k, gx.nk = n;
   gx.out = dx;
+  gx.tail = b.tail;
   gw.p = dz, gw.q = px.src ? px.dst : x, gw.ldp = ldz, gw.ldq = px.src ? padded(k, dtype) : ldx;
   gw.np = n, gw.nq = k, gw.nk = m;
   gw.out = dw;

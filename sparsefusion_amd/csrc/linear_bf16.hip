@@ -8,6 +8,6 @@ int sf_gemm_bf16(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
 int sf_gradients_bf16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
   return sf_gradients_go<__bf16>(dx, dw, db, st);
 }
-int sf_tiny_gradients_bf16(const SfGradients &g, bool whole, hipStream_t st) {
-  return sf_tiny_gradients_go<__bf16>(g, whole, st);
+int sf_tiny_gradients_bf16(const SfGradients &g, bool direct, hipStream_t st) {
+  return sf_tiny_gradients_go<__bf16>(g, direct, st);
 }

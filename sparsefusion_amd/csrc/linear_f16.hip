@@ -8,6 +8,6 @@ int sf_gemm_f16(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
 int sf_gradients_f16(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
   return sf_gradients_go<_Float16>(dx, dw, db, st);
 }
-int sf_tiny_gradients_f16(const SfGradients &g, bool whole, hipStream_t st) {
-  return sf_tiny_gradients_go<_Float16>(g, whole, st);
+int sf_tiny_gradients_f16(const SfGradients &g, bool direct, hipStream_t st) {
+  return sf_tiny_gradients_go<_Float16>(g, direct, st);
 }

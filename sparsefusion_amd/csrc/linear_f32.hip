@@ -8,6 +8,6 @@ int sf_gemm_f32(const SfGemmArgs &a, int layout, int tile, hipStream_t st) {
 int sf_gradients_f32(const SfGemmArgs &dx, const SfGemmArgs &dw, const SfColumnSums &db, hipStream_t st) {
   return sf_gradients_go<float>(dx, dw, db, st);
 }
-int sf_tiny_gradients_f32(const SfGradients &g, bool whole, hipStream_t st) {
-  return sf_tiny_gradients_go<float>(g, whole, st);
+int sf_tiny_gradients_f32(const SfGradients &g, bool direct, hipStream_t st) {
+  return sf_tiny_gradients_go<float>(g, direct, st);
 }

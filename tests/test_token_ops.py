@@ -213,10 +213,11 @@ def test_c_entry_points_refuse_bad_arguments():
     assert L.sf_linear(one, 8192, one, None, None, one, None, 80, 8192, 64, 0, 0, one, need - 1, None) == -2
     assert b'workspace' in L.sf_last_error()
     assert L.sf_linear_workspace(one, 64, one, 80, 64, 64, 0, 0) == 0
-    need = L.sf_linear_workspace(one + 4, 64, one, 80, 64, 64, 0, 0)      # a copy of x
-    assert need >= 80 * 64 * 4
-    assert L.sf_linear(one + 4, 64, one, None, None, one, None, 80, 64, 64, 0, 0, one, need - 1, None) == -2
-    assert L.sf_linear(one + 4, 64, one, None, None, one, None, 80, 64, 64, 0, 0, one + 4, need, None) == -1
+    assert L.sf_linear_workspace(one + 4, 67, one, 80, 64, 64, 0, 0) == 0
+    need = L.sf_linear_workspace(one, 65, one, 80, 64, 64, 1, 0)      # a copy of x
+    assert need >= 80 * 64 * 2
+    assert L.sf_linear(one, 65, one, None, None, one, None, 80, 64, 64, 1, 0, one, need - 1, None) == -2
+    assert L.sf_linear(one, 65, one, None, None, one, None, 80, 64, 64, 1, 0, one + 4, need, None) == -1
     assert b'aligned' in L.sf_last_error()
     assert L.sf_linear_backward(one, one, 8, one, None, one, one, one, 4, 8, 4, 0, 2, None, 0, None) == -1
     need = L.sf_linear_backward_workspace(one, one, 32, one, 6400, 32, 32, 2, 2)
@@ -264,11 +265,14 @@ SIZES = [(1, 64, 64), (1, 1, 1), (3, 7, 5), (64, 64, 64), (65, 127, 63), (129, 1
          (16, 72, 48), (17, 33, 31), (64, 1023, 65), (65, 3, 2)]
 # enough tiles for the larger shapes, whole, split and cut at the edges
 LARGE = [(4000, 512, 1024), (9000, 1024, 1000), (16300, 800, 1016), (2000, 4096, 4096)]
+# rows that end inside a 16-byte chunk: one step of k and many, whole and in parts, each shape of tile
+CUT = [(20001, 30, 514), (7002, 90, 1030), (300, 4098, 70), (3000, 2050, 202), (9001, 1027, 1001),
+       (40, 66, 2050), (6, 4098, 34), (500, 62, 62)]
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('m,k,n', SIZES + LARGE)
+@pytest.mark.parametrize('m,k,n', SIZES + LARGE + CUT)
 def test_linear_matches_float64(dev, dtype, m, k, n):
     x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev, scale=k ** -0.5)
     b, r = rand(3, n, dtype=dtype, dev=dev), rand(4, m, n, dtype=dtype, dev=dev)
@@ -281,7 +285,7 @@ def test_linear_matches_float64(dev, dtype, m, k, n):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
-@pytest.mark.parametrize('m,k,n', SIZES + LARGE + [(40000, 72, 48), (33, 300, 1111), (40000, 64, 1024)])
+@pytest.mark.parametrize('m,k,n', SIZES + LARGE + CUT + [(40000, 72, 48), (33, 300, 1111), (40000, 64, 1024)])
 def test_linear_backward_matches_float64(dev, dtype, m, k, n):
     x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev, scale=k ** -0.5)
     dy, z = rand(3, m, n, dtype=dtype, dev=dev), rand(4, m, n, dtype=dtype, dev=dev)
@@ -369,6 +373,30 @@ def test_linear_infinities_and_nan_stay_in_their_rows(dev, dtype):
                                   device=dev).repeat(m * 70)[:int((z <= 0).sum())]
         got, want = linear_backward(dy, x, w, z, 'relu'), linear_backward(masked, x, w, z, 'relu')
         assert all(torch.equal(p, q) and torch.isfinite(p).all() for p, q in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('m,k,n', [(130, 62, 70), (3000, 94, 602), (20001, 30, 514), (300, 4098, 70), (5, 30, 34)])
+def test_linear_nothing_leaks_behind_a_cut_row(dev, dtype, m, k, n):
+    """Rows that end inside a chunk lie against the next row's first values: those may be anything."""
+    x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev)
+    dy = rand(3, m, n, dtype=dtype, dev=dev)
+    bad = torch.arange(m, device=dev) % 3 == 1
+    x2, w2, dy2 = x.clone(), w.clone(), dy.clone()
+    x2[bad, 0], dy2[bad, 0] = float('nan'), float('inf')
+    y, y2 = linear(x, w), linear(x2, w)
+    assert torch.equal(y2[~bad], y[~bad]) and y2[bad].isnan().all()
+    odd = torch.arange(n, device=dev) % 3 == 1
+    w2[odd, :1] = float('nan')
+    y2 = linear(x, w2)
+    assert torch.equal(y2[:, ~odd], y[:, ~odd]) and y2[:, odd].isnan().all()
+    dx, dx2 = linear_backward(dy, x, w)[0], linear_backward(dy2, x, w)[0]
+    assert torch.equal(dx2[~bad], dx[~bad]) and not torch.isfinite(dx2[bad]).any()
+    # behind the last row: a view of a larger tensor whose rest is not finite
+    room = torch.full((m * k + 64,), float('nan'), dtype=dtype, device=dev)
+    room[:m * k] = x.flatten()
+    assert torch.equal(linear(room[:m * k].view(m, k), w), y)
 
 
 @pytest.mark.gpu
