@@ -292,7 +292,8 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   auto small = [&](long long np, long long nq, long long nk) {
     const long long bk = 128 / (long long)sf_dtype_size(dtype), steps = (nk + bk - 1) / bk;
     const long long t = ((np + 31) / 32) * ((nq + 31) / 32);
-    return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype, false)};
+    // workgroups that are not resident from the start cost theirs
+    return Plan{32, 1, steps * bk, tile_cost(32, t, steps, dtype, false) + (t > kMostSmallTiles ? t / 512.0 : 0)};
   };
   // Three ways, by cost (us, each launch 3): dz (and db's parts) by a pass of its own, then the two products
   // in one launch each; or both in one launch of 32 x 32 tiles, the one in the other's idle CUs; or these
@@ -307,12 +308,14 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   b.pair = k > 0 && m < (1 << 20) && x32.cost + w32.cost < b.dx.cost + b.dw.cost + 4;
   const long long bk = 128 / (long long)sf_dtype_size(dtype), tq = (k + 31) / 32;
   const double sx = (double)((n + bk - 1) / bk), sw = (double)((m + bk - 1) / bk);
-  const double work = ((double)((m + 31) / 32 * tq) * sx + (double)((n + 31) / 32 * tq) * sw) / 256;
+  const double tx = (double)((m + 31) / 32 * tq), tw = (double)((n + 31) / 32 * tq);
+  const double work = (tx * sx + tw * sw) / 256;
   const double longest = sx > sw ? sx : sw;
   const double step = dtype == SF_DTYPE_F32
                           ? !all ? 0.85 : act == SF_ACT_NONE ? 0.38 : act == SF_ACT_RELU ? 0.45 : 0.52
                           : !all ? 1.4 : act == SF_ACT_NONE ? 0.25 : act == SF_ACT_RELU ? 0.42 : 0.7;
-  const double tiny = 3 + step * (work > longest ? work : longest);
+  const double filled = step * work + (tx + tw > kMostSmallTiles ? (tx + tw - kMostSmallTiles) / 256 : 0);
+  const double tiny = 3 + (filled > step * longest ? filled : step * longest);
   b.tiny = k > 0 && work < 1000 && longest < 1000 && tiny < (b.pair ? pair : two);
   if (b.tiny) {
     b.bytes = 0;
