@@ -483,10 +483,10 @@ __device__ __forceinline__ void sf_unroll(F &&f) {
 }
 
 // Shape of a kernel: BP x BQ outputs by WP x WQ waves, steps of STEP bytes of k in a ring of RING
-// buffers, WGS workgroups to a CU; RES: a residual may be added.
-template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_, bool RES_ = true>
+// buffers, WGS workgroups to a CU.  RES: a residual may be added.  TAIL: clears what is behind cut rows.
+template <int BP_, int BQ_, int WP_, int WQ_, int STEP_, int RING_, int WGS_, bool RES_ = true, bool TAIL_ = false>
 struct SfShape {
-  static constexpr bool RES = RES_, TAIL = BP_ < 256;      // TAIL: clears what is behind cut rows
+  static constexpr bool RES = RES_, TAIL = TAIL_;
   static constexpr int BP = BP_, BQ = BQ_, WP = WP_, WQ = WQ_, STEP = STEP_, RING = RING_, WGS = WGS_;
   static constexpr int WAVES = WP * WQ, BYTES = (BP + BQ) * STEP, LDS = RING * BYTES + WAVES * 4096;
   static_assert(LDS * WGS <= 160 * 1024 && (RING == 2 || RING == 4), "LDS of a CU");
@@ -912,12 +912,12 @@ static int sf_gemm_go(const SfGemmArgs &a, hipStream_t st) {
 // residual 259200 x 1024 -> 256 takes 200 and 204, 32400 x 256 -> 1024 56 and 59.
 typedef SfShape<256, 256, 2, 4, 64, 4, 1> SfTile256;
 typedef SfShape<256, 256, 2, 4, 128, 2, 1, false> SfTile256Plain;
-typedef SfShape<128, 128, 2, 2, 128, 2, 2> SfTile128;
+template <bool TAIL> using SfTile128 = SfShape<128, 128, 2, 2, 128, 2, 2, true, TAIL>;
 // 64 x 64: deep enough to cover the latency of one workgroup alone (64 x 4096 -> 4096 bf16: 33 us with a
 // ring of 2, 21 with 4); fp32's products cover it themselves, three workgroups level the CUs better
 // (35344 x 512 -> 512: 164 us against 168).
-typedef SfShape<64, 64, 2, 2, 128, 4, 2> SfTile64;
-typedef SfShape<64, 64, 2, 2, 128, 2, 3> SfTile64Three;
+template <typename T, bool TAIL>
+using SfTile64 = SfShape<64, 64, 2, 2, 128, sizeof(T) == 4 ? 2 : 4, sizeof(T) == 4 ? 3 : 2, true, TAIL>;
 
 template <typename T, bool PMINOR, bool QMINOR>
 static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
@@ -929,9 +929,13 @@ static int sf_gemm_launch(const SfGemmArgs &a, int tile, hipStream_t st) {
     if constexpr (!PMINOR && !QMINOR)      // gradients have no residual
       if (a.residual && a.splits == 1) return sf_gemm_go<T, PMINOR, QMINOR, SfTile256>(a, st);
     rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile256Plain>(a, st);
-  } else if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128>(a, st);
-  else if constexpr (sizeof(T) == 4) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64Three>(a, st);
-  else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64>(a, st);
+  } else if (PMINOR || !a.tail) {
+    if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128<false>>(a, st);
+    else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64<T, false>>(a, st);
+  } else if constexpr (!PMINOR) {
+    if (tile == 128) rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile128<true>>(a, st);
+    else rc = sf_gemm_go<T, PMINOR, QMINOR, SfTile64<T, true>>(a, st);
+  }
   if (rc) return rc;
   if (a.splits > 1) sf_gemm_join<T>(a, st);
   return SF_OK;
