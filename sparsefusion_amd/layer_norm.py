@@ -6,6 +6,9 @@ whose forward runs `sf_layer_norm` (csrc/layer_norm.hip); it is registered as th
 blocks apply it to the (N, C) voxel features).  Rows are fp32, fp16 or bf16, parameters of the same
 type or fp32; statistics and sums are fp32 and every output is rounded once.  Differentiable once (no
 double backward).  No CPU path.
+
+Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
+over the same leaves may be alive outside the capture.
 """
 import torch
 from torch import nn
