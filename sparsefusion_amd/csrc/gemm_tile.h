@@ -37,48 +37,64 @@ typedef short sf_s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// Phi(z), the normal distribution function, as 1 / (1 + exp(-z P(z^2))): P fits logit(Phi(z)) / z
-// over |z| <= 6, its coefficients (by powers of z^2) for the least maximal error of Phi; the leading
-// one is positive, so farther out Phi runs into 0 or 1.  fp32: seven coefficients, 2.9e-8 off (half a
-// step of fp32 at 1 is 6e-8); 16-bit outputs: five, 1.4e-6 off (half a step of fp16 at 1 is 2.4e-4).
-// 18 and 16 instruction slots (exp and rcp take four each) against about 45 of
-// 0.5 (1 + erff(z / sqrt(2))), whose two branches both run in most waves: the layer of
-// 32400 x 256 -> 1024 went from 68 to 47 us with it.  With the fp32 evaluation 1.3e-7 and 1.6e-6 off.
-// The coefficients carry -log2(e) for v_exp_f32.
+// GELU, z Phi(z), from the side where Phi is small: with a = |z|, Phi(-a) = exp(-a^2 / 2) M(a), where M (Mills'
+// ratio over sqrt(2 pi)) is t Q(t) of t = 1 / (1 + p a); then gelu(z) = max(z, 0) - a Phi(-a) keeps its digits
+// for negative z too, where gelu is far smaller than z.  Q is fitted for the least maximal error of M, weighted
+// so that in 16 bits Phi(-a) is off by at most 1e-6 and by 6e-5 of itself up to a = 4 (a quarter of half an fp16
+// step), 4e-4 farther out (where fp16 has no digits left; a fifth of half a bf16 step): five coefficients.  fp32:
+// seven, 5.2e-8 of itself up to a = 1 and 5.2e-8 (1 + (a - 1)^3) beyond, where the exponent's rounding, 2.5 a^2
+// times 2^-24, is as much.  a stops at 14, where Phi(-a) is below the smallest normal number: an infinite
+// z comes out as infinity or 0, and NaN stays (the minimum hands it on).  20 and 22 instruction slots (exp and rcp
+// take four each); a logistic form, whose error is absolute, 16 and 18, 0.5 (1 + erff(z / sqrt(2))) about 45.
 template <typename T>
-__device__ __forceinline__ float sf_phi(float z) {
-  constexpr float kL = -1.4426950408889634f;
-  const float q = z * z;
-  float p;
+__device__ __forceinline__ float sf_mills(float a) {
+  float q;
   if constexpr (sizeof(T) == 4) {
-    p = 3.51255832e-09f * kL;
-    p = fmaf(p, q, -2.64532672e-07f * kL);
-    p = fmaf(p, q, 7.92954762e-06f * kL);
-    p = fmaf(p, q, -1.10612640e-04f * kL);
-    p = fmaf(p, q, -6.51894754e-05f * kL);
-    p = fmaf(p, q, 7.26661688e-02f * kL);
-    p = fmaf(p, q, 1.59576988e+00f * kL);
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.34f, 1.0f));
+    q = 4.56890270e-02f;
+    q = fmaf(q, t, -2.04008249e-01f);
+    q = fmaf(q, t, 2.69765421e-01f);
+    q = fmaf(q, t, -3.55146202e-02f);
+    q = fmaf(q, t, 1.58752532e-01f);
+    q = fmaf(q, t, 1.29248573e-01f);
+    q = fmaf(q, t, 1.36067344e-01f);
+    return q * t;
   } else {
-    p = 2.85001296e-06f * kL;
-    p = fmaf(p, q, -7.33869147e-05f * kL);
-    p = fmaf(p, q, -1.75652994e-04f * kL);
-    p = fmaf(p, q, 7.27845723e-02f * kL);
-    p = fmaf(p, q, 1.59573942e+00f * kL);
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.35f, 1.0f));
+    q = -9.57236643e-02f;
+    q = fmaf(q, t, 2.69671341e-01f);
+    q = fmaf(q, t, 2.51945219e-02f);
+    q = fmaf(q, t, 1.63298806e-01f);
+    q = fmaf(q, t, 1.37559687e-01f);
+    return q * t;
   }
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(p * z));
+}
+__device__ __forceinline__ float sf_gauss(float a) {      // exp(-a^2 / 2)
+  const float b = a * 0.84932180028801905f;
+  return __builtin_amdgcn_exp2f(-(b * b));
+}
+__device__ __forceinline__ float sf_tail(float z) { return __builtin_elementwise_minimum(__builtin_fabsf(z), 14.0f); }
+template <typename T>
+__device__ __forceinline__ float sf_gelu(float z) {
+  const float a = sf_tail(z);
+  return fmaf(-a, sf_gauss(a) * sf_mills<T>(a), fmaxf(z, 0.0f));
+}
+// Phi(z) + z phi(z): 1 - s for s of -z
+template <typename T>
+__device__ __forceinline__ float sf_gelu_slope(float z) {
+  const float a = sf_tail(z), s = sf_gauss(a) * fmaf(a, -0.39894228040143268f, sf_mills<T>(a));
+  return z < 0.0f ? s : 1.0f - s;
 }
 template <typename T>
 __device__ __forceinline__ float sf_act(float z, int act) {
   if (act == SF_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (act == SF_ACT_GELU) return z * sf_phi<T>(z);
+  if (act == SF_ACT_GELU) return sf_gelu<T>(z);
   return z;
 }
 template <typename T>
 __device__ __forceinline__ float sf_act_gradient(float g, float z, int act) {
   if (act == SF_ACT_RELU) return z <= 0.0f ? 0.0f : g;      // whatever g is
-  if (act == SF_ACT_GELU)      // Phi(z) + z phi(z)
-    return g * fmaf(z * 0.39894228040143268f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f),
-                    sf_phi<T>(z));
+  if (act == SF_ACT_GELU) return g * sf_gelu_slope<T>(z);
   return g;
 }
 

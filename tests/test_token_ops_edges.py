@@ -1,0 +1,112 @@
+"""Token operators where a bound on the average case sees nothing: digits of small values, sums whose
+parts can be told apart, inputs that are not plain memory, calls that cannot be served.
+
+Tolerances count half steps of the storage type (u), E = 2^-24 for an fp32 operation, and what the
+kernels' own approximations state; each is derived where it stands.
+"""
+import math
+
+import pytest
+import torch
+
+from sparsefusion_amd.linear import linear, linear_backward, linear_forward
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+IDS = ['f32', 'f16', 'bf16']
+E = 2.0 ** -24
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+
+
+def rand(seed, *shape, dtype=torch.float32, dev='cpu', scale=1.0, shift=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale + shift).to(dtype).to(dev)
+
+
+# ---------------------------------------------------------------------------------- digits of GELU
+
+def gelu_inputs(dtype, dev):
+    """Every 16-bit number of [-20, 20] that is not subnormal; for fp32 a grid of 2^-11, and powers of two
+    around zero."""
+    if dtype == torch.float32:
+        z = torch.arange(-20 * 2048, 20 * 2048 + 1, device=dev).float() / 2048
+        small = 2.0 ** torch.arange(-120, 0, device=dev).float()
+        z = torch.cat([z, small, -small])
+    else:
+        z = torch.arange(-32768, 32768, dtype=torch.int32, device=dev).to(torch.int16).view(dtype)
+    z = z[(z.abs() <= 20) & ((z.abs() >= torch.finfo(dtype).smallest_normal) | (z == 0))]
+    return torch.cat([z, z.new_zeros(-z.numel() % 64)]).view(-1, 64)
+
+
+def gelu_bounds(z, dtype):
+    """-> gelu, its slope and what each may be off by before it is rounded to dtype.  Phi(-a), a = |z|, is
+    off by `fit` of itself; exp(-a^2 / 2) by 2.5 a^2 E (the constant and the two products in its exponent)
+    and 2 E; the reciprocal 2 E, seven steps of a Horner scheme whose terms add up to twice its value 28 E,
+    products 4 E.  Results below the smallest normal fp32 number may be flushed."""
+    zd = z.double()
+    a = zd.abs()
+    tail = torch.special.erfc(a / math.sqrt(2)) / 2      # (ndtr loses its digits for arguments far below 0)
+    density = torch.exp(-a * a / 2) / math.sqrt(2 * math.pi)
+    if dtype == torch.float32:
+        fit = 5.2e-8 * (1 + (a - 1).clamp(min=0) ** 3)
+    else:
+        fit = torch.where(a <= 4, 6e-5, 4e-4)
+    rel = fit + (2.5 * a * a + 36) * E
+    flush = 20 * torch.finfo(torch.float32).smallest_normal
+    y = torch.where(zd < 0, -a * tail, zd - a * tail)
+    s = tail - a * density
+    slope = torch.where(zd < 0, s, 1 - s)
+    return (y, a * tail * rel + E * y.abs() + flush,
+            slope, tail * rel + a * density * (2.5 * a * a + 8) * E + 2 * E * slope.abs() + flush)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('rows,width', [(8, 64), (None, 64), (20000, 512)])
+def test_gelu_keeps_the_digits_of_its_type(dev, dtype, rows, width):
+    """Through an identity weight (its products and sums are exact): few rows, tiny and large layers."""
+    z = gelu_inputs(dtype, dev)
+    if width > 64:
+        z = z.reshape(-1)[torch.arange(rows * width, device=dev) % z.numel()].view(rows, width)
+    eye = torch.eye(width, dtype=dtype, device=dev)
+    dy = torch.where(torch.arange(z.numel(), device=dev).view_as(z) % 3 == 1, -1.5, 1.0).to(dtype)
+    for part in ((z,) if width > 64 or rows is None else z.split(rows)):
+        y, ey, slope, es = gelu_bounds(part, dtype)
+        got, pre = linear_forward(part, eye, None, 'gelu', None, True)
+        assert torch.equal(pre, part)
+        over = (got.double() - y).abs() - (ey + u(dtype) * (y.abs() + ey) + tiny(dtype))
+        worst = over.argmax()
+        assert over.max() <= 0, (part.flatten()[worst].item(), got.flatten()[worst].item(), y.flatten()[worst].item())
+        if rows == 8 and width == 64:
+            continue
+        g = dy.double()
+        dx, _, _ = linear_backward(dy, part, eye, part, 'gelu', (True, False, False))
+        want, err = g * slope, g.abs() * (es + E * slope.abs())
+        over = (dx.double() - want).abs() - (err + u(dtype) * (want.abs() + err) + tiny(dtype))
+        worst = over.argmax()
+        assert over.max() <= 0, (part.flatten()[worst].item(), dx.flatten()[worst].item(), want.flatten()[worst].item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+def test_gelu_of_infinities_and_nan(dev, dtype):
+    inf = float('inf')
+    big = torch.finfo(dtype).max
+    z = torch.tensor([inf, -inf, float('nan'), big, -big, 0.0], dtype=dtype, device=dev)[:, None]
+    for m in (6, 600):
+        x = z.repeat(m // 6, 1)
+        one = torch.ones(1, 1, dtype=dtype, device=dev)
+        y = linear(x, one, activation='gelu').view(-1, 6)
+        assert (y[:, 0] == inf).all() and not y[:, 1].any() and y[:, 2].isnan().all()
+        assert (y[:, 3] == big).all() and not y[:, 4].any() and not y[:, 5].any()
+        dy = torch.ones_like(x)
+        dx = linear_backward(dy, x, one, x, 'gelu', (True, False, False))[0].view(-1, 6)
+        want = torch.tensor([1, 0, float('nan'), 1, 0, 0.5], dtype=dtype, device=dev)
+        assert torch.equal(dx.isnan(), want.isnan().expand_as(dx))
+        assert torch.equal(dx.nan_to_num(), want.nan_to_num().expand_as(dx))
