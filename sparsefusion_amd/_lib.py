@@ -8,6 +8,7 @@ import os
 import subprocess
 
 import torch
+from torch.autograd import forward_ad
 
 _raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream wraps
 _get_device = torch._C._cuda_getDevice
@@ -201,6 +202,13 @@ def same(x, name, t):
     """Refuse a tensor of another type or on another device than x."""
     if t.dtype != x.dtype or t.device != x.device:
         raise RuntimeError(f'{name} must be {x.dtype} on {x.device}, got {t.dtype} on {t.device}')
+
+
+def refuse_tangents(op, *tensors):
+    """Called inside a forward-mode level (forward_ad._current_level >= 0): a raw pointer carries no tangent,
+    and an output without one would count as constant."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f'{op} has no forward-mode derivative')
 
 
 def rows(x):

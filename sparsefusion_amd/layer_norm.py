@@ -5,7 +5,8 @@ whose forward runs `sf_layer_norm` (csrc/layer_norm.hip); it is registered as th
 `norm_cfg=dict(type='LN')` reaches it in every module that builds its norms from a config (sparse conv
 blocks apply it to the (N, C) voxel features).  Rows are fp32, fp16 or bf16, parameters of the same
 type or fp32; statistics and sums are fp32 and every output is rounded once.  Differentiable once (no
-double backward).  No CPU path.
+double backward) and backwards only: tensors with forward-mode tangents are refused, and so is
+torch.jit.trace.  No CPU path.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
@@ -29,6 +30,8 @@ def _check(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise RuntimeError(f'layer_norm needs rows of at least one element, got {tuple(x.shape)}')
     d = x.shape[-1]
+    if type(d) is not int:      # torch.jit.trace hands out tensors, and would record allocations, no call
+        raise RuntimeError('layer_norm cannot be traced')
     if d > MOST_FEATURES:
         raise RuntimeError(f'layer_norm takes rows of up to {MOST_FEATURES} elements, got {d}')
     pdtype = None
@@ -51,6 +54,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, retur
     """-> (y, sum, mean, rstd) of s = x + residual, y = (s - mean) * rstd * weight + bias.  sum (s
     rounded) with return_sum, mean and rstd (fp32, x.shape[:-1]) with keep_stats, else None.  Not
     differentiable: see `layer_norm`."""
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents('layer_norm', x, weight, bias, residual)
     d, code, pdtype = _check(x, weight, bias)
     if not eps >= 0:
         raise RuntimeError(f'eps must not be negative, got {eps}')
@@ -90,6 +95,8 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, grad_sum=None, needs=(
     `grad_sum` of the sum (or None); x is the normalised sum, mean and rstd as it returned them.  dx is
     the gradient of x and of the residual alike.  `needs` says which are wanted, the others are None;
     the parameter gradients have weight's type (without a weight: `param_dtype`, or x's)."""
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents('layer_norm_backward', grad, x, mean, rstd, weight, grad_sum)
     d, code, pdtype = _check(x, weight, None)
     if weight is None and param_dtype is not None:
         pdtype = param_dtype

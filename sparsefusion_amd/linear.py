@@ -3,7 +3,8 @@
 `Linear` is `nn.Linear` (same arguments, parameters and state-dict keys) whose forward runs
 `sf_linear` (csrc/linear.hip, csrc/gemm_tile.h); `FeedForward` is the two-layer block of the decoders
 that read the BEV map.  fp32, fp16 and bf16, all tensors of a call of one type; products and sums are
-fp32 and every output is rounded once.  Differentiable once (no double backward).  No CPU path.
+fp32 and every output is rounded once.  Differentiable once (no double backward) and backwards only: tensors
+with forward-mode tangents are refused, and so is torch.jit.trace.  No CPU path.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
@@ -34,6 +35,8 @@ def _check(x, weight, device):
     if weight.dim() != 2:
         raise RuntimeError(f'weight must be (out_features, in_features), got {tuple(weight.shape)}')
     n, k = weight.shape
+    if type(n) is not int:      # torch.jit.trace hands out tensors, and would record allocations, no call
+        raise RuntimeError('linear cannot be traced')
     if x.dim() < 1 or x.shape[-1] != k:
         raise RuntimeError(f'expected rows of {k} elements, got {tuple(x.shape)}')
     if n > MOST_FEATURES or k > MOST_FEATURES:
@@ -50,6 +53,8 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
     act = ACTIVATIONS.get(activation)
     if act is None:
         act = _act_code(activation)
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents('linear', x, weight, bias, residual)
     device = x.device
     n, k, code = _check(x, weight, device)
     shape = (x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n)
@@ -94,6 +99,8 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     output; `pre` as it returned them (not needed without an activation).  `needs` says which are
     wanted, the others are None.  The residual's gradient is `grad` itself."""
     act = _act_code(activation)
+    if _lib.forward_ad._current_level >= 0:
+        _lib.refuse_tangents('linear_backward', grad, x, weight, pre)
     n, k, code = _check(x, weight, x.device)
     shape = (*x.shape[:-1], n)
     if not act:

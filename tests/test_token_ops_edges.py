@@ -9,7 +9,8 @@ import math
 import pytest
 import torch
 
-from sparsefusion_amd.linear import linear, linear_backward, linear_forward
+from sparsefusion_amd.layer_norm import layer_norm, layer_norm_backward, layer_norm_forward
+from sparsefusion_amd.linear import Linear, linear, linear_backward, linear_forward
 
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 IDS = ['f32', 'f16', 'bf16']
@@ -110,3 +111,40 @@ def test_gelu_of_infinities_and_nan(dev, dtype):
         want = torch.tensor([1, 0, float('nan'), 1, 0, 0.5], dtype=dtype, device=dev)
         assert torch.equal(dx.isnan(), want.isnan().expand_as(dx))
         assert torch.equal(dx.nan_to_num(), want.nan_to_num().expand_as(dx))
+
+
+# ---------------------------------------------------------------------------------- calls that cannot be served
+
+def test_forward_mode_tangents_are_refused():
+    """Without a HIP device: the refusal comes before the device is looked at, plain tensors get that far."""
+    from torch.autograd import forward_ad
+    x, w, b = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8)
+    stats = torch.zeros(4)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: linear(dual(x), w, b), lambda: linear(x, dual(w), b), lambda: linear(x, w, dual(b)),
+                     lambda: linear(x, w, b, residual=dual(x)), lambda: linear_forward(dual(x), w),
+                     lambda: linear_backward(dual(x), x, w), lambda: linear_backward(x, dual(x), w),
+                     lambda: linear_backward(x, x, w, dual(x), 'relu'),
+                     lambda: layer_norm(dual(x)), lambda: layer_norm(x, dual(b)), lambda: layer_norm(x, b, dual(b)),
+                     lambda: layer_norm(x, residual=dual(x)), lambda: layer_norm_forward(dual(x)),
+                     lambda: layer_norm_backward(dual(x), x, stats, stats),
+                     lambda: layer_norm_backward(x, x, stats, stats, None, dual(x))):
+            with torch.no_grad(), pytest.raises(RuntimeError, match='no forward-mode derivative'):
+                call()
+        for call in (lambda: linear(x, w, b), lambda: layer_norm(x, b)):
+            with pytest.raises(RuntimeError, match='HIP device'):
+                call()
+        # parameters that require grad: the autograd function has no forward-mode rule either
+        with pytest.raises(RuntimeError):
+            Linear(8, 8)(dual(x))
+
+
+def test_traces_are_refused():
+    x, w, b = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8)
+    for call in (lambda t: linear(t, w, b), lambda t: linear_backward(t, x, w)[0], lambda t: layer_norm(t, b),
+                 lambda t: layer_norm_backward(t, x, b[:4], b[:4])[0], Linear(8, 8)):
+        with pytest.raises(RuntimeError, match='cannot be traced'):
+            torch.jit.trace(call, x)
