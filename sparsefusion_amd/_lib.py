@@ -211,6 +211,13 @@ def refuse_tangents(op, *tensors):
         raise RuntimeError(f'{op} has no forward-mode derivative')
 
 
+def resolved(*tensors):
+    """The tensors, lazily negated ones (the imaginary part of a conjugate) written out: their memory holds the
+    other sign.  Their elements are two apart, so that only one of a single element, or rows of one, pass
+    for what a kernel may read in place: callers ask at those sizes (0.2 us a tensor)."""
+    return [t.resolve_neg() if t is not None and t.is_neg() else t for t in tensors]
+
+
 def rows(x):
     """(..., K) as (M, K) with adjacent elements and evenly spaced rows, and their distance; a copy
     only where the strides do not allow a view."""

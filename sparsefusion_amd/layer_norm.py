@@ -57,6 +57,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, retur
     if _lib.forward_ad._current_level >= 0:
         _lib.refuse_tangents('layer_norm', x, weight, bias, residual)
     d, code, pdtype = _check(x, weight, bias)
+    if d == 1:
+        x, weight, bias, residual = _lib.resolved(x, weight, bias, residual)
     if not eps >= 0:
         raise RuntimeError(f'eps must not be negative, got {eps}')
     if residual is not None:
@@ -108,6 +110,8 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, grad_sum=None, needs=(
             if t.shape != x.shape:
                 raise RuntimeError(f'{name} must have shape {tuple(x.shape)}, got {tuple(t.shape)}')
     m = x.numel() // d
+    if d == 1 or m == 1:
+        grad, x, mean, rstd, weight, grad_sum = _lib.resolved(grad, x, mean, rstd, weight, grad_sum)
     for name, t in (('mean', mean), ('rstd', rstd)):
         if t.dtype != torch.float32 or t.numel() != m or t.device != x.device:
             raise RuntimeError(f'{name} must be {m} fp32 values on {x.device}, got {tuple(t.shape)} '

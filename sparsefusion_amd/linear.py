@@ -57,6 +57,8 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
         _lib.refuse_tangents('linear', x, weight, bias, residual)
     device = x.device
     n, k, code = _check(x, weight, device)
+    if k == 1 or n == 1:
+        x, weight, bias, residual = _lib.resolved(x, weight, bias, residual)
     shape = (x.shape[0], n) if x.dim() == 2 else (*x.shape[:-1], n)
     pb = pr = pp = None
     if bias is not None:
@@ -102,6 +104,8 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     if _lib.forward_ad._current_level >= 0:
         _lib.refuse_tangents('linear_backward', grad, x, weight, pre)
     n, k, code = _check(x, weight, x.device)
+    if k == 1 or n == 1:
+        grad, x, weight, pre = _lib.resolved(grad, x, weight, pre)
     shape = (*x.shape[:-1], n)
     if not act:
         pre = None

@@ -9,6 +9,7 @@ import math
 import pytest
 import torch
 
+from sparsefusion_amd import _lib
 from sparsefusion_amd.layer_norm import layer_norm, layer_norm_backward, layer_norm_forward
 from sparsefusion_amd.linear import Linear, linear, linear_backward, linear_forward
 
@@ -111,6 +112,52 @@ def test_gelu_of_infinities_and_nan(dev, dtype):
         want = torch.tensor([1, 0, float('nan'), 1, 0, 0.5], dtype=dtype, device=dev)
         assert torch.equal(dx.isnan(), want.isnan().expand_as(dx))
         assert torch.equal(dx.nan_to_num(), want.nan_to_num().expand_as(dx))
+
+
+# ---------------------------------------------------------------------------------- inputs that are no plain memory
+
+def negated(t):
+    """t as a lazily negated view: the imaginary part of a conjugate, 2 elements apart."""
+    view = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert view.is_neg() and torch.equal(view, t)
+    return view
+
+
+def test_lazily_negated_views_are_resolved():
+    """Contiguous, or rows of one element that rows() hands on as they are: only these need a look."""
+    for shape in ((1, 1), (5, 1), (1, 3), (3, 4), (1,), (2, 2, 1), (2, 2, 3)):
+        t = negated(rand(1, *shape))
+        assert t.is_contiguous() == (t.numel() == 1)
+        assert _lib.rows(t)[0].is_neg() == (shape[-1] == 1)
+        out, none, same = _lib.resolved(t, None, rand(2, 3))
+        assert not out.is_neg() and torch.equal(out, t) and none is None and torch.equal(same, rand(2, 3))
+
+
+@pytest.mark.gpu
+def test_lazily_negated_tensors(dev):
+    """Sizes at which such a view keeps the strides that the kernels read in place (fp32: complex numbers)."""
+    for m, k, n in ((5, 1, 7), (1, 1, 1), (300, 1, 64), (6, 8, 1)):
+        x, w, b, r = (rand(i, *s, dev=dev) for i, s in enumerate(((m, k), (n, k), (n,), (m, n))))
+        dy, z = rand(5, m, n, dev=dev), rand(6, m, n, dev=dev)
+        y = linear(x, w, b, 'gelu', r)
+        assert torch.equal(linear(*map(negated, (x, w, b)), 'gelu', negated(r)), y)
+        want = linear_backward(dy, x, w, z, 'gelu')
+        got = linear_backward(*map(negated, (dy, x, w, z)), 'gelu')
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        if n == 1:      # a gradient that autograd hands over in this form
+            xl = x.clone().requires_grad_()
+            out = linear(xl, w, b)
+            torch.complex(torch.zeros_like(out), out).conj().imag.backward(dy)
+            assert torch.equal(xl.grad, linear_backward(-dy, x, w)[0])
+    for m, d in ((4, 1), (1, 1), (3, 8)):
+        x, r, dy, ds = (rand(i, m, d, dev=dev, shift=0.5) for i in range(4))
+        w, b = rand(7, d, dev=dev), rand(8, d, dev=dev)
+        y, s, mean, rstd = layer_norm_forward(x, w, b, 1e-5, r, True, True)
+        got = layer_norm_forward(*map(negated, (x, w, b)), 1e-5, negated(r), True, True)
+        assert all(torch.equal(p, q) for p, q in zip(got, (y, s, mean, rstd)))
+        want = layer_norm_backward(dy, s, mean, rstd, w, ds)
+        got = layer_norm_backward(*map(negated, (dy, s, mean, rstd, w, ds)))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
 # ---------------------------------------------------------------------------------- calls that cannot be served
