@@ -10,8 +10,10 @@ import subprocess
 import torch
 from torch.autograd import forward_ad
 
-_raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream wraps
-_get_device = torch._C._cuda_getDevice
+# what torch.cuda.current_stream and current_device wrap; a torch without devices has neither, and its host
+# side (configurations, module definitions, sizes of workspaces) goes without
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)
+_get_device = getattr(torch._C, '_cuda_getDevice', None)
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libsparsefusion_hip.so')
 _LIB = None

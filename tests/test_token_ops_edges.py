@@ -5,6 +5,9 @@ Tolerances count half steps of the storage type (u), E = 2^-24 for an fp32 opera
 kernels' own approximations state; each is derived where it stands.
 """
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -195,3 +198,26 @@ def test_traces_are_refused():
                  lambda t: layer_norm_backward(t, x, b[:4], b[:4])[0], Linear(8, 8)):
         with pytest.raises(RuntimeError, match='cannot be traced'):
             torch.jit.trace(call, x)
+
+
+# ---------------------------------------------------------------------------------- the package around them
+
+def test_import_needs_no_device_functions():
+    """A torch built without devices lacks the bindings that the stream and device lookups use."""
+    code = """
+import torch
+for name in ('_cuda_getCurrentRawStream', '_cuda_getDevice'):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import sparsefusion_amd
+from sparsefusion_amd import _lib, layer_norm, linear, pipeline, sparse_encoder, voxelize
+try:
+    linear.linear(torch.zeros(2, 3), torch.zeros(4, 3))
+except RuntimeError as e:
+    assert 'HIP device' in str(e), e
+else:
+    raise SystemExit('served')
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
