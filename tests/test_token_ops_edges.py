@@ -221,3 +221,12 @@ else:
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+@pytest.mark.gpu
+def test_stream_of_any_form_of_device(dev):
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for device in (dev, torch.device('cuda', 0), torch.device('cuda'), 0, 'cuda:0', 'cuda', None):
+            assert _lib.stream(device) == side.cuda_stream
+    assert _lib.stream(0) == torch.cuda.current_stream().cuda_stream
