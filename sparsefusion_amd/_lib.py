@@ -19,7 +19,6 @@ LIB_PATH = os.path.join(_HERE, 'libsparsefusion_hip.so')
 _LIB = None
 
 SF_OK = 0
-SF_ERR_WORKSPACE = -2
 
 _vp, _i, _sz, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_longlong
 _F3, _F6, _I3 = C.c_float * 3, C.c_float * 6, C.c_int * 3   # array instances decay to pointers
@@ -137,6 +136,10 @@ def lib():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
+        # Touches the library's thread-local storage.  Until a thread has touched that of the library loaded
+        # last, glibc looks up every thread-local of the others (torch reads some in each call) the slow way:
+        # gradients of 400 x 256 -> 128 fp32 13.2 us a call without, 11.3 with.
+        L.sf_last_error()
         _LIB = L
     return _LIB
 

@@ -9,6 +9,8 @@ with forward-mode tangents are refused, and so is torch.jit.trace.  No CPU path.
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
 """
+import functools
+
 import torch
 from torch import nn
 
@@ -44,6 +46,18 @@ def _check(x, weight, device):
     if weight.dtype != dtype or weight.device != device:
         _lib.same(x, 'weight', weight)
     return n, k, code
+
+
+# Scratch bytes by sizes and by where in 16 bytes the operands start: plans depend on nothing else, and asking
+# anew costs a call twice what looking them up does.
+@functools.lru_cache(maxsize=4096)
+def _forward_scratch(x_at, ldx, weight_at, m, k, n, code, residual):
+    return _lib.lib().sf_linear_workspace(x_at, ldx, weight_at, m, k, n, code, residual)
+
+
+@functools.lru_cache(maxsize=4096)
+def _backward_scratch(grad_at, x_at, ldx, weight_at, m, k, n, code, act):
+    return _lib.lib().sf_linear_backward_workspace(grad_at, x_at, ldx, weight_at, m, k, n, code, act)
 
 
 def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pre=False):
@@ -84,13 +98,10 @@ def linear_forward(x, weight, bias=None, activation=None, residual=None, keep_pr
         pre = x.new_empty(shape)
         pp = pre.data_ptr()
     m, px, pw, py, stream = rows.shape[0], rows.data_ptr(), weight.data_ptr(), y.data_ptr(), _lib.stream(device)
-    L = _lib.lib()
-    # most sizes need no scratch: only a refusal asks how much
-    rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, None, 0, stream)
-    if rc == _lib.SF_ERR_WORKSPACE:
-        nbytes = L.sf_linear_workspace(px, ldx, pw, m, k, n, code, pr is not None)
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-        rc = L.sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, ws.data_ptr(), nbytes, stream)
+    nbytes = _forward_scratch(px & 15, ldx, pw & 15, m, k, n, code, pr is not None)
+    ws = _lib.workspace(nbytes, x)
+    rc = _lib.lib().sf_linear(px, ldx, pw, pb, pr, py, pp, m, k, n, code, act, None if ws is None else ws.data_ptr(),
+                              nbytes, stream)
     if rc:
         _lib.check(rc)
     return y, pre
@@ -127,16 +138,13 @@ def linear_backward(grad, x, weight, pre=None, activation=None, needs=(True, Tru
     dx = x.new_empty(x.shape) if needs[0] else None
     dw = x.new_empty((n, k)) if needs[1] else None
     db = x.new_empty(n) if needs[2] else None
-    L = _lib.lib()
     pg, px, pw = grad.data_ptr(), rows.data_ptr(), weight.data_ptr()
-    args = (pg, px, ldx, pw, None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
-            None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code, act)
-    stream = _lib.stream(x.device)
-    rc = L.sf_linear_backward(*args, None, 0, stream)      # tiny layers need no scratch
-    if rc == _lib.SF_ERR_WORKSPACE:
-        nbytes = L.sf_linear_backward_workspace(pg, px, ldx, pw, m, k, n, code, act)
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-        rc = L.sf_linear_backward(*args, ws.data_ptr(), nbytes, stream)
+    nbytes = _backward_scratch(pg & 15, px & 15, ldx, pw & 15, m, k, n, code, act)
+    ws = _lib.workspace(nbytes, x)
+    rc = _lib.lib().sf_linear_backward(
+        pg, px, ldx, pw, None if pre is None else pre.data_ptr(), None if dx is None else dx.data_ptr(),
+        None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(), m, k, n, code, act,
+        None if ws is None else ws.data_ptr(), nbytes, _lib.stream(x.device))
     if rc:
         _lib.check(rc)
     return dx, dw, db

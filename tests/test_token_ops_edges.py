@@ -230,3 +230,46 @@ def test_stream_of_any_form_of_device(dev):
         for device in (dev, torch.device('cuda', 0), torch.device('cuda'), 0, 'cuda:0', 'cuda', None):
             assert _lib.stream(device) == side.cuda_stream
     assert _lib.stream(0) == torch.cuda.current_stream().cuda_stream
+
+
+def test_scratch_depends_on_sizes_and_places_alone():
+    """What the Python layer looks up by sizes and by the operands' place in 16 bytes is what the library asks
+    for at the addresses themselves."""
+    L = _lib.lib()
+    for code in (0, 1, 2):
+        for m, k, n in ((1, 64, 64), (80, 8192, 64), (80, 65, 64), (6400, 32, 33), (3001, 451, 333), (40000, 256, 256)):
+            for place in (0, 2, 4, 8, 14):
+                at = [0x7f0000000000 + 4096 * i + place for i in range(3)]
+                low = [a & 15 for a in at]
+                for res in (0, 1):
+                    assert (L.sf_linear_workspace(at[0], k, at[1], m, k, n, code, res) ==
+                            L.sf_linear_workspace(low[0], k, low[1], m, k, n, code, res))
+                    assert (L.sf_linear_backward_workspace(at[0], at[1], k, at[2], m, k, n, code, res) ==
+                            L.sf_linear_backward_workspace(low[0], low[1], k, low[2], m, k, n, code, res))
+
+
+@pytest.mark.gpu
+def test_calls_are_made_once(dev, monkeypatch):
+    """No call is refused on the way to its result, and a message that a caller has yet to read stays."""
+    L = _lib.lib()
+    assert L.sf_linear(64, 8, 64, None, None, 64, None, 4, 8, 4, 7, 0, None, 0, None) == -1
+    told = L.sf_last_error()
+    calls = []
+
+    class Counted:
+        def __getattr__(self, name):
+            calls.append(name)
+            return getattr(L, name)
+
+    monkeypatch.setattr(_lib, 'lib', Counted)
+    for m, k, n in ((4, 8, 6), (80, 8192, 64), (81, 65, 33), (6400, 32, 32), (2000, 1024, 1024)):
+        for dtype in DTYPES:
+            x, w = rand(1, m, k, dtype=dtype, dev=dev), rand(2, n, k, dtype=dtype, dev=dev)
+            dy = rand(3, m, n, dtype=dtype, dev=dev)
+            for _ in range(2):
+                calls.clear()
+                linear(x, w, activation='relu')
+                linear_backward(dy, x, w, dy, 'gelu')
+                assert calls.count('sf_linear') == 1 and calls.count('sf_linear_backward') == 1
+            assert len(calls) == 2      # known sizes ask for nothing more
+    assert L.sf_last_error() == told
