@@ -5,9 +5,11 @@
 //   dw = sum_rows dy xh;  db = sum_rows dy
 //
 // Both directions are bound by memory: every tensor is read or written once, the row lives in
-// registers between its loads (all in flight at once) and its stores (the variance is the centred second
-// pass over those registers, so a large common offset costs no digits; the mean is summed from s / d, so
-// rows whose sum passes fp32's range keep theirs), and all sums are fp32.  259200 x 256 bf16, 531 MB each
+// registers between its loads (all in flight at once) and its stores, and all sums are fp32.  The mean is
+// summed from s / d, so rows whose sum passes fp32's range keep theirs; it is off by some steps of a large
+// common offset.  A second pass over the registers sums what is left of the row, c = s - mu (exact for values
+// near mu), and its squares: mean(c) corrects the mean, mean(c^2) - mean(c)^2 is the variance, and the offset
+// costs no digits (a row of 1000 times 1000.7 gave up to 0.04 without, 0 with).  259200 x 256 bf16, 531 MB each
 // way: add and norm 92 us (5.8 TB/s), gradients 91 us and 5 for the join; a copy of that size moves
 // 4.9 TB/s.
 //
@@ -44,6 +46,29 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
   return v;
 }
 
+// The same for two sums at once.
+template <int LANES, int THREADS>
+__device__ __forceinline__ void group_sums(float &a, float &b, float (*red)[2]) {
+#pragma unroll
+  for (int d = (LANES < 64 ? LANES : 64) / 2; d > 0; d >>= 1) {
+    const float u = __shfl_xor(a, d, 64), v = __shfl_xor(b, d, 64);
+    a += u, b += v;
+  }
+  if constexpr (LANES > 64) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][0] = a, red[threadIdx.x >> 6][1] = b;
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) a += red[i][0], b += red[i][1];
+  }
+}
+
+// mean(c^2) - mean(c)^2, which rounding may carry below 0; NaN stays.
+__device__ __forceinline__ float variance(float mean_square, float mean) {
+  return __builtin_elementwise_maximum(fmaf(-mean, mean, mean_square), 0.0f);
+}
+
 template <typename P, int V>
 __device__ __forceinline__ void load_param(const void *p, int i0, int n, float fallback, float *v) {
   // parameters may be fp32 beside 16-bit rows, so their chunk is V elements of their own type
@@ -58,7 +83,7 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
                 T *__restrict__ y, T *__restrict__ sum, float *__restrict__ mean,
                 float *__restrict__ rstd, long long m, int d, float eps) {
   constexpr int V = SfChunk<T>::V, GROUPS = THREADS / LANES;
-  __shared__ float red[16];
+  __shared__ float red[16], red2[16][2];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const float inv_d = 1.0f / (float)d;
   float wv[NV][V], bv[NV][V];
@@ -92,24 +117,26 @@ norm_fwd_kernel(const T *__restrict__ x, const T *__restrict__ res, const void *
       for (int j = 0; j < V; ++j) s = fmaf(v[c][j], inv_d, s);   // zeros behind the row's end
     }
     const float mu = group_sum<LANES, THREADS>(s, red);
-    float q = 0.0f;
+    float q = 0.0f, e = 0.0f;
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         v[c][j] -= mu;
-        if ((c * LANES + lane) * V + j < d) q += v[c][j] * v[c][j];
+        if ((c * LANES + lane) * V + j < d) q += v[c][j] * v[c][j], e += v[c][j];
       }
-    const float rs = 1.0f / sqrtf(group_sum<LANES, THREADS>(q, red) * inv_d + eps);
+    group_sums<LANES, THREADS>(q, e, red2);
+    e *= inv_d;
+    const float rs = 1.0f / sqrtf(variance(q * inv_d, e) + eps);
     if (!live) continue;
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[c][j] = v[c][j] * rs * wv[c][j] + bv[c][j];
+      for (int j = 0; j < V; ++j) v[c][j] = (v[c][j] - e) * rs * wv[c][j] + bv[c][j];
       sf_store_chunk<T, MODE == SF_STREAM>(y + at, (c * LANES + lane) * V, d, v[c]);
     }
     if (lane == 0) {
-      if (mean) mean[row] = mu;
+      if (mean) mean[row] = mu + e;
       if (rstd) rstd[row] = rs;
     }
   }
@@ -122,7 +149,7 @@ norm_fwd_long_kernel(const T *__restrict__ x, const T *__restrict__ res, const v
                      T *__restrict__ y, T *__restrict__ sum, float *__restrict__ mean,
                      float *__restrict__ rstd, long long m, int d, float eps) {
   constexpr int V = SfChunk<T>::V;
-  __shared__ float red[16];
+  __shared__ float red[16], red2[16][2];
   const float inv_d = 1.0f / (float)d;
   for (long long row = blockIdx.x; row < m; row += gridDim.x) {
     const long long at = row * d;
@@ -135,7 +162,7 @@ norm_fwd_long_kernel(const T *__restrict__ x, const T *__restrict__ res, const v
         for (int j = 0; j < V; ++j) v[j] += u[j];
       }
     };
-    float s = 0.0f, q = 0.0f, v[V];
+    float s = 0.0f, q = 0.0f, e = 0.0f, v[V];
     for (long long i0 = threadIdx.x * V; i0 < d; i0 += 1024 * V) {
       load((int)i0, v);
       if (sum) sf_store_chunk<T>(sum + at, i0, d, v);
@@ -147,20 +174,22 @@ norm_fwd_long_kernel(const T *__restrict__ x, const T *__restrict__ res, const v
       load((int)i0, v);
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (i0 + j < d) q += (v[j] - mu) * (v[j] - mu);
+        if (i0 + j < d) q += (v[j] - mu) * (v[j] - mu), e += v[j] - mu;
     }
-    const float rs = 1.0f / sqrtf(group_sum<1024, 1024>(q, red) * inv_d + eps);
+    group_sums<1024, 1024>(q, e, red2);
+    e *= inv_d;
+    const float rs = 1.0f / sqrtf(variance(q * inv_d, e) + eps);
     for (long long i0 = threadIdx.x * V; i0 < d; i0 += 1024 * V) {
       float wv[V], bv[V];
       load_param<P, V>(w, (int)i0, d, 1.0f, wv);
       load_param<P, V>(b, (int)i0, d, 0.0f, bv);
       load((int)i0, v);
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = (v[j] - mu) * rs * wv[j] + bv[j];
+      for (int j = 0; j < V; ++j) v[j] = (v[j] - mu - e) * rs * wv[j] + bv[j];
       sf_store_chunk<T>(y + at, i0, d, v);
     }
     if (threadIdx.x == 0) {
-      if (mean) mean[row] = mu;
+      if (mean) mean[row] = mu + e;
       if (rstd) rstd[row] = rs;
     }
   }

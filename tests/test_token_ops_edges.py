@@ -117,6 +117,57 @@ def test_gelu_of_infinities_and_nan(dev, dtype):
         assert torch.equal(dx.nan_to_num(), want.nan_to_num().expand_as(dx))
 
 
+# ---------------------------------------------------------------------------------- digits of layer norm
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('d', [1, 7, 40, 128, 320, 333, 700, 1000, 1500, 3000, 5000, 16000, 20001])
+def test_a_common_offset_costs_no_digits(dev, dtype, d):
+    """Rows far from zero, with little spread or none.  A sum's error is ge = (d / 64 + 48) E of the magnitudes;
+    the first mean's, dm, is that of the offset; what is left of a value, at most |s - m| + dm, is centred by
+    the mean of all that is left, off by ge of those magnitudes, with two roundings of E.  The variance carries
+    twice that error times the spread, its square, and ge; rstd half of its relative error and 4 E."""
+    rows = [torch.full((d,), c) for c in (0.0, 0.1, 100.0, 1000.7, -12345.6, 3.0e4)]
+    rows += [c + spread * rand(i, d) for i, (c, spread) in enumerate(
+        [(1000.0, 1e-3), (250.0, 1.0), (-3000.0, 0.01), (2.0e4, 30.0), (1.0, 1e-3), (0.0, 1.0)])]
+    x = torch.stack(rows).to(dtype).to(dev)
+    w, b = rand(20, d, dtype=dtype, dev=dev, shift=1.0), rand(21, d, dtype=dtype, dev=dev)
+    ge = (d / 64 + 48) * E
+    s = x.double()
+    m = s.mean(1, keepdim=True)
+    dm = ge * s.abs().mean(1, keepdim=True)
+    left = (s - m).abs() + dm
+    dc = ge * left.mean(1, keepdim=True) + 2 * E * left
+    for eps in (1e-5, 1e-3):
+        y, _, mean, rstd = layer_norm_forward(x, w, b, eps, keep_stats=True)
+        var = (s - m).square().mean(1, keepdim=True)
+        r = 1 / torch.sqrt(var + eps)
+        # squares of what is left: ge and its own roundings of them, the offset's share cancels to as much
+        dv = 2 * var.sqrt() * dc.square().mean(1, keepdim=True).sqrt() + dc.square().mean(1, keepdim=True) \
+            + (ge + 4 * E) * left.square().mean(1, keepdim=True) + 2 * dm * ge * left.mean(1, keepdim=True)
+        dr = r * (0.5 * dv * r * r * (1 + dv * r * r) + 4 * E)
+        xh = (s - m) * r
+        dxh = dc * (r + dr) + (s - m).abs() * dr + 2 * E * xh.abs()
+        want = xh * w.double() + b.double()
+        err = dxh * w.double().abs() + 2 * E * (xh * w.double()).abs() + E * want.abs()
+        bound = err + u(dtype) * (want.abs() + err) + tiny(dtype)
+        over = (y.double() - want).abs() - bound
+        assert over.max() <= 0, (divmod(over.argmax().item(), d), (y.double() - want).abs().max(1).values)
+        assert ((mean.double() - m[:, 0]).abs() <= (dc.mean(1) + 2 * E * m[:, 0].abs() + 1e-45)).all()
+        assert ((rstd.double() - r[:, 0]).abs() <= (dr + 2 * E * r)[:, 0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('d', [64, 320, 3000, 20001])
+def test_a_constant_row_normalises_to_its_bias(dev, d):
+    """To a part in 1e5 (fp32, eps 1e-5): what is left of the offset is within ge^2 rstd of it."""
+    ge = (d / 64 + 48) * E
+    b = rand(1, d, dev=dev)
+    for c in (1000.7, -77.3, 0.1):
+        y = layer_norm(torch.full((3, d), c, device=dev), None, b)
+        assert (y - b).abs().max() <= 2 * ge * ge * abs(c) * 317 + 1e-6
+
+
 # ---------------------------------------------------------------------------------- inputs that are no plain memory
 
 def negated(t):
