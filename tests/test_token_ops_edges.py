@@ -168,6 +168,83 @@ def test_a_constant_row_normalises_to_its_bias(dev, d):
         assert (y - b).abs().max() <= 2 * ge * ge * abs(c) * 317 + 1e-6
 
 
+# ---------------------------------------------------------------------------------- sums, exactly
+
+def whole(seed, *shape, dtype=torch.float32, dev='cpu'):
+    """-2, -1, 1 or 2: products and their sums are exact in fp32, in any order, as long as they stay below 2^24,
+    and no term is 0, so that none can be left out without a trace."""
+    g = torch.Generator().manual_seed(seed)
+    return torch.tensor([-2.0, -1.0, 1.0, 2.0])[torch.randint(0, 4, shape, generator=g)].to(dtype).to(dev)
+
+
+def assert_sum(got, want, what):
+    """want (float64) is exact: got is it, rounded once."""
+    want = want.to(got.dtype)
+    wrong = (got != want).nonzero()
+    assert not len(wrong), (what, len(wrong), wrong[0].tolist(), got[tuple(wrong[0])].item(), want[tuple(wrong[0])].item())
+
+
+def linear_sums(dy, x, w, keep=slice(None)):
+    """dx, dw and db in 64 bits; `keep`: of these rows alone (dx: all)."""
+    dy, x, w = dy.double(), x.double(), w.double()
+    return dy @ w, dy[keep].T @ x[keep], dy[keep].sum(0)
+
+
+def norm_sums(dy, x, mean, rstd, keep=slice(None)):
+    xh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    return (dy.double() * xh)[keep].sum(0), dy.double()[keep].sum(0)
+
+
+def test_exact_sums_show_what_is_left_out():
+    """The comparisons below turn down sums without the last row, a run of rows or a share of them."""
+    assert set(whole(1, 4000).tolist()) == {-2.0, -1.0, 1.0, 2.0}
+    m = 70000
+    dy, x, y, w = whole(1, m, 5), whole(2, m, 6), whole(6, m, 5), whole(3, 5, 6)
+    mean, rstd = whole(4, m), 2.0 ** whole(5, m)
+    rows = torch.arange(m)
+    for left in (rows == m - 1, rows == 0, rows >= m - 128, rows % 97 == 5, (rows >= 640) & (rows < 704)):
+        for name, full, part in (*zip(('dw', 'db'), linear_sums(dy, x, w)[1:], linear_sums(dy, x, w, ~left)[1:]),
+                                 *zip(('dw', 'db'), norm_sums(dy, y, mean, rstd), norm_sums(dy, y, mean, rstd, ~left))):
+            assert_sum(full.float(), full, name)
+            with pytest.raises(AssertionError):
+                assert_sum(part.float(), full, name)
+
+
+SUM_SIZES = [(1, 64, 64), (7, 5, 3), (65, 127, 63), (200, 128, 256), (1000, 512, 512), (4000, 512, 1024),
+             (2000, 4096, 96), (16300, 800, 1016), (20001, 30, 514), (40000, 72, 48), (9001, 1027, 1001),
+             (33, 300, 1111), (32400, 256, 256), (70001, 64, 40), (110000, 33, 37), (259200, 64, 64), (6, 8192, 40)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('m,k,n', SUM_SIZES)
+def test_linear_sums_are_complete(dev, dtype, m, k, n):
+    x, w, b = whole(1, m, k, dtype=dtype, dev=dev), whole(2, n, k, dtype=dtype, dev=dev), whole(3, n, dtype=dtype, dev=dev)
+    dy, z = whole(4, m, n, dtype=dtype, dev=dev), whole(5, m, n, dtype=dtype, dev=dev)
+    assert_sum(linear(x, w, b), x.double() @ w.double().T + b.double(), 'y')
+    for act, g in ((None, dy), ('relu', dy * (z > 0))):
+        for needs in ((True, True, True), (False, True, False), (False, False, True)):
+            for name, got, want in zip(('dx', 'dw', 'db'), linear_backward(dy, x, w, z, act, needs), linear_sums(g, x, w)):
+                if got is not None:
+                    assert_sum(got, want, (name, act, needs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES, ids=IDS)
+@pytest.mark.parametrize('m,d', [(1, 64), (3, 7), (200, 128), (5003, 333), (5000, 96), (1537, 2048), (515, 4097), (64, 16384),
+                                 (100, 20001), (70000, 40), (110000, 333), (70000, 512), (259200, 64)])
+def test_layer_norm_sums_are_complete(dev, dtype, m, d):
+    """Statistics handed over that keep (x - mean) * rstd exact."""
+    x, dy = whole(1, m, d, dtype=dtype, dev=dev), whole(2, m, d, dtype=dtype, dev=dev)
+    mean, rstd = whole(3, m, dev=dev), 2.0 ** whole(4, m, dev=dev)
+    for pd in {dtype, torch.float32}:
+        w = whole(5, d, dtype=pd, dev=dev)
+        _, dw, db = layer_norm_backward(dy, x, mean, rstd, w, dy)
+        assert dw.dtype == db.dtype == pd
+        for name, got, want in zip(('dw', 'db'), (dw, db), norm_sums(dy, x, mean, rstd)):
+            assert_sum(got, want, name)
+
+
 # ---------------------------------------------------------------------------------- inputs that are no plain memory
 
 def negated(t):
