@@ -218,6 +218,17 @@ def refuse_tangents(op, *tensors):
         raise RuntimeError(f'{op} has no forward-mode derivative')
 
 
+dispatch_modes = torch._C._len_torch_dispatch_stack
+
+
+def refuse_tracing(op):
+    """Called inside dispatch modes (dispatch_modes() > 0): those that record operators (make_fx, export) see an
+    output's allocation and not the call that fills it, fake tensors have no memory.  Modes that watch are fine."""
+    key = torch._C._TorchDispatchModeKey
+    if any(torch._C._get_dispatch_mode(k) is not None for k in (key.PROXY, key.FAKE, key.FUNCTIONAL)):
+        raise RuntimeError(f'{op} cannot be traced')
+
+
 def resolved(*tensors):
     """The tensors, lazily negated ones (the imaginary part of a conjugate) written out: their memory holds the
     other sign.  Their elements are two apart, so that only one of a single element, or rows of one, pass

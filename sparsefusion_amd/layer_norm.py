@@ -6,7 +6,7 @@ whose forward runs `sf_layer_norm` (csrc/layer_norm.hip); it is registered as th
 blocks apply it to the (N, C) voxel features).  Rows are fp32, fp16 or bf16, parameters of the same
 type or fp32; statistics and sums are fp32 and every output is rounded once.  Differentiable once (no
 double backward) and backwards only: tensors with forward-mode tangents are refused, and so is
-torch.jit.trace.  No CPU path.
+torch.jit.trace, make_fx and export.  No CPU path.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
@@ -32,6 +32,8 @@ def _check(x, weight, bias):
     d = x.shape[-1]
     if type(d) is not int:      # torch.jit.trace hands out tensors, and would record allocations, no call
         raise RuntimeError('layer_norm cannot be traced')
+    if _lib.dispatch_modes():
+        _lib.refuse_tracing('layer_norm')
     if d > MOST_FEATURES:
         raise RuntimeError(f'layer_norm takes rows of up to {MOST_FEATURES} elements, got {d}')
     pdtype = None

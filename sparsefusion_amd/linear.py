@@ -4,7 +4,7 @@
 `sf_linear` (csrc/linear.hip, csrc/gemm_tile.h); `FeedForward` is the two-layer block of the decoders
 that read the BEV map.  fp32, fp16 and bf16, all tensors of a call of one type; products and sums are
 fp32 and every output is rounded once.  Differentiable once (no double backward) and backwards only: tensors
-with forward-mode tangents are refused, and so is torch.jit.trace.  No CPU path.
+with forward-mode tangents are refused, and so is torch.jit.trace, make_fx and export.  No CPU path.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
@@ -39,6 +39,8 @@ def _check(x, weight, device):
     n, k = weight.shape
     if type(n) is not int:      # torch.jit.trace hands out tensors, and would record allocations, no call
         raise RuntimeError('linear cannot be traced')
+    if _lib.dispatch_modes():
+        _lib.refuse_tracing('linear')
     if x.dim() < 1 or x.shape[-1] != k:
         raise RuntimeError(f'expected rows of {k} elements, got {tuple(x.shape)}')
     if n > MOST_FEATURES or k > MOST_FEATURES:

@@ -328,6 +328,32 @@ def test_traces_are_refused():
             torch.jit.trace(call, x)
 
 
+def test_recorded_operators_are_refused():
+    """make_fx in each of its modes, and fake tensors; a mode that only watches is none of them."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    x, w, b, stats = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8), torch.zeros(4)
+    calls = (lambda t: linear(t, w, b), lambda t: linear_backward(t, t, w)[0], lambda t: layer_norm(t, b),
+             lambda t: layer_norm_backward(t, t, stats, stats)[0], Linear(8, 8))
+    for call in calls:
+        for mode in ('real', 'fake', 'symbolic'):
+            with pytest.raises(RuntimeError, match='cannot be traced'):
+                make_fx(call, tracing_mode=mode)(x)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        for call in calls[:4]:
+            with pytest.raises(RuntimeError, match='cannot be traced'):
+                call(mode.from_tensor(x))
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    for call in calls:
+        with Watch(), pytest.raises(RuntimeError, match='HIP device'):
+            call(x)
+
+
 # ---------------------------------------------------------------------------------- the package around them
 
 def test_import_needs_no_device_functions():
