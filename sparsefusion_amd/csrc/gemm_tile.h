@@ -37,17 +37,23 @@ typedef short sf_s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned sf_u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// GELU, z Phi(z), from the side where Phi is small: with a = |z|, Phi(-a) = exp(-a^2 / 2) M(a), where M (Mills'
-// ratio over sqrt(2 pi)) is t Q(t) of t = 1 / (1 + p a); then gelu(z) = max(z, 0) - a Phi(-a) keeps its digits
-// for negative z too, where gelu is far smaller than z.  Q is fitted for the least maximal error of M, weighted
-// so that in 16 bits Phi(-a) is off by at most 1e-6 and by 6e-5 of itself up to a = 4 (a quarter of half an fp16
-// step), 4e-4 farther out (where fp16 has no digits left; a fifth of half a bf16 step): five coefficients.  fp32:
-// seven, 5.2e-8 of itself up to a = 1 and 5.2e-8 (1 + (a - 1)^3) beyond, where the exponent's rounding, 2.5 a^2
-// times 2^-24, is as much.  a stops at 14, where Phi(-a) is below the smallest normal number: an infinite
-// z comes out as infinity or 0, and NaN stays (the minimum hands it on).  20 and 22 instruction slots (exp and rcp
-// take four each); a logistic form, whose error is absolute, 16 and 18, 0.5 (1 + erff(z / sqrt(2))) about 45.
+// GELU, z Phi(z), from the side where Phi is small: with a = |z|, gelu(z) = max(z, 0) - a Phi(-a) keeps its digits
+// for negative z too, where it is far smaller than z.  Phi(-a) is fitted for the least maximal error relative to
+// itself.  16 bits: 2^P(a), P the polynomial of degree 9 nearest to log2(Phi(-a)) up to 13, off by at most 8e-7,
+// 5e-5 of itself up to a = 4 (a fifth of half an fp16 step) and 3.5e-4 farther out, where fp16 has no digits left (a
+// sixth of half a bf16 step).  fp32, where P's terms would round to more: exp(-a^2 / 2) M(a), M (Mills' ratio over
+// sqrt(2 pi)) = t Q(t) of t = 1 / (1 + 0.34 a) with seven coefficients, off by 5.2e-8 of itself up to a = 1 and
+// 5.2e-8 (1 + (a - 1)^3) beyond, where the exponent's rounding, 2.5 a^2 times 2^-24, is as much.
+// a stops at 14, where both come out as 0 (v_exp_f32 flushes what is below the smallest normal number): an infinite
+// z gives infinity or 0, and NaN stays (minimum and maximum hand it on).  32400 x 256 -> 1024 bf16, 24.4 us without an
+// activation: 34.8 us, with a quotient of degrees 4 and 2 for P 36.5, with fmaxf, which takes two instructions, 2.3
+// more, with a logistic form, whose error is absolute (4.5 % of gelu(-4)), 34.3.
+__device__ __forceinline__ float sf_gauss(float a) {      // exp(-a^2 / 2)
+  const float b = a * 0.84932180028801905f;
+  return __builtin_amdgcn_exp2f(-(b * b));
+}
 template <typename T>
-__device__ __forceinline__ float sf_mills(float a) {
+__device__ __forceinline__ float sf_phi_below(float a) {      // Phi(-a)
   float q;
   if constexpr (sizeof(T) == 4) {
     const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.34f, 1.0f));
@@ -58,31 +64,31 @@ __device__ __forceinline__ float sf_mills(float a) {
     q = fmaf(q, t, 1.58752532e-01f);
     q = fmaf(q, t, 1.29248573e-01f);
     q = fmaf(q, t, 1.36067344e-01f);
-    return q * t;
+    return sf_gauss(a) * (q * t);
   } else {
-    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.35f, 1.0f));
-    q = -9.57236643e-02f;
-    q = fmaf(q, t, 2.69671341e-01f);
-    q = fmaf(q, t, 2.51945219e-02f);
-    q = fmaf(q, t, 1.63298806e-01f);
-    q = fmaf(q, t, 1.37559687e-01f);
-    return q * t;
+    q = -6.95180746e-10f;
+    q = fmaf(q, a, 7.87926524e-08f);
+    q = fmaf(q, a, -3.26799250e-06f);
+    q = fmaf(q, a, 7.15041460e-05f);
+    q = fmaf(q, a, -9.55835043e-04f);
+    q = fmaf(q, a, 8.49724654e-03f);
+    q = fmaf(q, a, -5.38178124e-02f);
+    q = fmaf(q, a, -4.58641291e-01f);
+    q = fmaf(q, a, -1.15119171e+00f);
+    q = fmaf(q, a, -9.99997973e-01f);
+    return __builtin_amdgcn_exp2f(q);
   }
 }
-__device__ __forceinline__ float sf_gauss(float a) {      // exp(-a^2 / 2)
-  const float b = a * 0.84932180028801905f;
-  return __builtin_amdgcn_exp2f(-(b * b));
-}
-__device__ __forceinline__ float sf_tail(float z) { return __builtin_elementwise_minimum(__builtin_fabsf(z), 14.0f); }
+__device__ __forceinline__ float sf_below(float z) { return __builtin_elementwise_minimum(__builtin_fabsf(z), 14.0f); }
 template <typename T>
 __device__ __forceinline__ float sf_gelu(float z) {
-  const float a = sf_tail(z);
-  return fmaf(-a, sf_gauss(a) * sf_mills<T>(a), fmaxf(z, 0.0f));
+  const float a = sf_below(z);
+  return fmaf(-a, sf_phi_below<T>(a), __builtin_elementwise_maximum(z, 0.0f));
 }
 // Phi(z) + z phi(z): 1 - s for s of -z
 template <typename T>
 __device__ __forceinline__ float sf_gelu_slope(float z) {
-  const float a = sf_tail(z), s = sf_gauss(a) * fmaf(a, -0.39894228040143268f, sf_mills<T>(a));
+  const float a = sf_below(z), s = fmaf(a * -0.39894228040143268f, sf_gauss(a), sf_phi_below<T>(a));
   return z < 0.0f ? s : 1.0f - s;
 }
 template <typename T>
