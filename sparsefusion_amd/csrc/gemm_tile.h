@@ -1055,7 +1055,7 @@ __device__ __forceinline__ void sf_store_shared(const sf_f32x16 &acc, unsigned c
 // is no pass ahead and nothing to copy: loads need no alignment, and what is outside reads as zeros.
 // 32 x 32 tiles, a step's 128 bytes of k shared by the four waves, DEEP steps' loads in flight.  Bound by
 // the step: 0.4 us in fp32, in GELU's slope 0.5 (16 bits 0.7), one wave a SIMD.  400 x 256 -> 128 fp32 ReLU
-// 8.2 us, 200 x 256 -> 256 bf16 GELU 5.4; with a pass for dz ahead 9.5 and 9.7, and a launch more.
+// 8.2 us, 200 x 256 -> 256 bf16 GELU 5.7; with a pass for dz ahead 9.5 and 9.7, and a launch more.
 template <typename T, bool DW, bool DIRECT>
 __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned char *lds, int group) {
   constexpr int B = 32, STEP = 128, V = 16 / sizeof(T), BK = STEP / (int)sizeof(T), DEEP = 4;
@@ -1144,17 +1144,22 @@ __device__ __forceinline__ void sf_tiny_db(const SfGradients &g, float *red, int
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.0f;
   for (long long r = rl; r < g.m; r += RL * DEEP) {
-    frag e[DEEP], z[DEEP];
+    frag e[DEEP], z[DEEP] = {};
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
       e[i] = sf_row_chunk<T>(dy, g.n, r + i * RL, col < g.n ? g.m : 0, col, g.n);
       if (g.act != SF_ACT_NONE) z[i] = sf_row_chunk<T>(pre, g.n, r + i * RL, col < g.n ? g.m : 0, col, g.n);
     }
+    auto add = [&](auto act) {      // one branch a turn: with one an element they run one behind the other
 #pragma unroll
-    for (int i = 0; i < DEEP; ++i)
+      for (int i = 0; i < DEEP; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        sum[j] += g.act != SF_ACT_NONE ? sf_act_gradient<T>((float)e[i][j], (float)z[i][j], g.act) : (float)e[i][j];
+        for (int j = 0; j < V; ++j)
+          sum[j] += sf_act_gradient<T>((float)e[i][j], (float)z[i][j], decltype(act)::value);
+    };
+    if (g.act == SF_ACT_GELU) add(SfInt<SF_ACT_GELU>());
+    else if (g.act == SF_ACT_RELU) add(SfInt<SF_ACT_RELU>());
+    else add(SfInt<SF_ACT_NONE>());
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) red[rl * 33 + cl * V + j] = sum[j];

@@ -298,7 +298,7 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   // Three ways, by cost (us, each launch 3): dz (and db's parts) by a pass of its own, then the two products
   // in one launch each; or both in one launch of 32 x 32 tiles, the one in the other's idle CUs; or these
   // tiles alone, making dz as they read dy.  That is work for each tile again (us a step below), worth it
-  // while the steps are few: 400 x 256 -> 128 fp32 ReLU 8.2 us (pass and pair 9.5), bf16 GELU 7.9 (10.1),
+  // while the steps are few: 400 x 256 -> 128 fp32 ReLU 8.2 us (pass and pair 9.5), bf16 GELU 7.6 (10.1),
   // 500 x 512 -> 512 bf16 ReLU 9.4 (11.8), GELU 14.2 (12.5), 1000 x 512 -> 512 fp32 GELU 35 (25).  With one
   // of the gradients asked for the tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
