@@ -503,7 +503,8 @@ SF_API int sf_dynamic_scatter(const float *feats, const int *coors, int n, int c
 #define SF_LINEAR_MOST_FEATURES (1 << 20)
 
 /* Bytes of scratch (16-byte aligned) sf_linear needs for these operands; 0 for most.  The pointers are
- * looked at, not followed: operands whose rows start at an odd number of 16-bit elements are copied first. */
+ * looked at, not followed, and only for their place in 16 bytes: operands whose rows start at an odd number of
+ * 16-bit elements are copied first. */
 SF_API size_t sf_linear_workspace(const void *x, long long ldx, const void *weight, long long m,
                                   long long k, long long n, int dtype, int has_residual);
 
@@ -516,7 +517,7 @@ SF_API int sf_linear(const void *x, long long ldx, const void *weight, const voi
                      const void *residual, void *y, void *pre, long long m, long long k, long long n,
                      int dtype, int act, void *workspace, size_t workspace_bytes, void *stream);
 
-/* Bytes of scratch (16-byte aligned) sf_linear_backward needs for these operands. */
+/* Bytes of scratch (16-byte aligned) sf_linear_backward needs for these operands (pointers as above). */
 SF_API size_t sf_linear_backward_workspace(const void *dy, const void *x, long long ldx,
                                            const void *weight, long long m, long long k, long long n,
                                            int dtype, int act);

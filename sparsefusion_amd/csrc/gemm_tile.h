@@ -308,9 +308,9 @@ __device__ __forceinline__ int sf_steps(const SfGemmArgs &a, int split) {
 
 // Epilogue of a wave's TP x TQ blocks of 32 x 32 at (p0, q0).  A block goes through the wave's own
 // 4 KB of LDS (quads of columns swizzled by the row) so that bias, pre, residual and output move in
-// whole 16-byte chunks of a row; the plain sums when the contraction is split.  Stripes of 32 rows are
-// a real loop (unrolled, the code of a large tile outgrows the instruction cache); the accumulators
-// cannot be indexed by it, so each block is picked by comparison.
+// whole 16-byte chunks of a row; the plain sums when the contraction is split.  Tiles whose rows and columns all
+// exist are straight-line code over all blocks (whole, sums), so that the next block's work runs under a
+// block's loads and stores; cut ones a loop over the blocks (ragged).
 template <typename T, int TP, int TQ>
 struct SfEpilogue {
   static constexpr int V = 16 / sizeof(T), CPL = 32 / V, RPT = 64 / CPL, ITS = 32 / RPT;
@@ -1055,7 +1055,7 @@ __device__ __forceinline__ void sf_store_shared(const sf_f32x16 &acc, unsigned c
 // is no pass ahead and nothing to copy: loads need no alignment, and what is outside reads as zeros.
 // 32 x 32 tiles, a step's 128 bytes of k shared by the four waves, DEEP steps' loads in flight.  Bound by
 // the step: 0.4 us in fp32, in GELU's slope 0.5 (16 bits 0.7), one wave a SIMD.  400 x 256 -> 128 fp32 ReLU
-// 8.2 us, 200 x 256 -> 256 bf16 GELU 5.7; with a pass for dz ahead 9.5 and 9.7, and a launch more.
+// 8.3 us, 200 x 256 -> 256 bf16 GELU 5.7; with a pass for dz ahead 10.2 and 9.8, and a launch more.
 template <typename T, bool DW, bool DIRECT>
 __device__ __forceinline__ void sf_tiny_gradient(const SfGradients &g, unsigned char *lds, int group) {
   constexpr int B = 32, STEP = 128, V = 16 / sizeof(T), BK = STEP / (int)sizeof(T), DEEP = 4;

@@ -298,8 +298,10 @@ BackwardPlan backward_plan(const void *dy, const void *x, long long ldx, const v
   // Three ways, by cost (us, each launch 3): dz (and db's parts) by a pass of its own, then the two products
   // in one launch each; or both in one launch of 32 x 32 tiles, the one in the other's idle CUs; or these
   // tiles alone, making dz as they read dy.  That is work for each tile again (us a step below), worth it
-  // while the steps are few: 400 x 256 -> 128 fp32 ReLU 8.2 us (pass and pair 9.5), bf16 GELU 7.6 (10.1),
-  // 500 x 512 -> 512 bf16 ReLU 9.4 (11.8), GELU 14.2 (12.5), 1000 x 512 -> 512 fp32 GELU 35 (25).  With one
+  // while the steps are few: 400 x 256 -> 128 fp32 ReLU 8.4 us (pass and pair 10.2), bf16 GELU 7.6 (10.1),
+  // 200 x 512 -> 512 bf16 ReLU 7.3 (10.0), but 1000 x 256 -> 256 bf16 GELU 13.2 (12.4), 1500 x 128 -> 128 fp32 GELU
+  // 28 (18.5).  In between ReLU and no activation take the pass too early, a full chip's steps being charged as
+  // much as a lone workgroup's: 500 x 512 -> 512 bf16 ReLU 11.4, and 7.8 in tiles.  With one
   // of the gradients asked for the tiles stay the same, so that its values do.
   const Plan x32 = small(m, k, n), w32 = small(n, k, m);
   const bool copy = !direct(x, ldx, dtype) || !direct(w, k, dtype), all = !copy && direct(dy, n, dtype);

@@ -75,10 +75,11 @@ __device__ __forceinline__ typename SfChunk<T>::type sf_load_raw(const T *__rest
 }
 
 // Whether m rows of `row_bytes` go around the caches, NT: tensors of 64 MB (the last-level cache holds
-// 256 MB, a pass has four such) whose rows are whole lines.  Without and with, no output written twice
-// to the same place: add and norm of 259200 x 256 bf16 104 and 98 us, of 60000 x 512 fp32 100 and 94, its
-// gradients 95 and 86; with rows that share lines (110000 x 333 fp32) 161 and 167, of cached tensors
-// (5003 x 333 fp32) 9.2 and 10.3.  (Measured before the row's loads went out together.)
+// 256 MB, a pass has four such) whose rows are whole lines.  In us without and with, inputs and outputs in other
+// places each time: add and norm of 259200 x 256 bf16 97 and 91, of 60000 x 512 fp32 90 and 86, their gradients 105
+// and 94, 96 and 87; the pass for dz of 32400 x 2048 bf16 and the products that read it 139 and 129.  At 32 MB the
+// norms still gain (65536 x 256 bf16 29.2 and 27.3), a dz that is read again loses (52.3 and 53.6).  Rows that share
+// lines: gradients of norms of 130000 x 200 fp32 79 and 73, but of 17000 x 2056 142 and 157.
 static inline bool sf_streamed(long long m, size_t row_bytes) {
   return row_bytes % 128 == 0 && (size_t)m * row_bytes >= ((size_t)64 << 20);
 }

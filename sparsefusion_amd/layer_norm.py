@@ -5,7 +5,7 @@ whose forward runs `sf_layer_norm` (csrc/layer_norm.hip); it is registered as th
 `norm_cfg=dict(type='LN')` reaches it in every module that builds its norms from a config (sparse conv
 blocks apply it to the (N, C) voxel features).  Rows are fp32, fp16 or bf16, parameters of the same
 type or fp32; statistics and sums are fp32 and every output is rounded once.  Differentiable once (no
-double backward) and backwards only: tensors with forward-mode tangents are refused, and so is
+double backward) and backwards only: tensors with forward-mode tangents are refused, and so are
 torch.jit.trace, make_fx and export.  No CPU path.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph

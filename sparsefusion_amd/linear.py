@@ -4,7 +4,11 @@
 `sf_linear` (csrc/linear.hip, csrc/gemm_tile.h); `FeedForward` is the two-layer block of the decoders
 that read the BEV map.  fp32, fp16 and bf16, all tensors of a call of one type; products and sums are
 fp32 and every output is rounded once.  Differentiable once (no double backward) and backwards only: tensors
-with forward-mode tangents are refused, and so is torch.jit.trace, make_fx and export.  No CPU path.
+with forward-mode tangents are refused, and so are torch.jit.trace, make_fx and export.  No CPU path.
+
+With an activation the gradient ahead of it, dz, is rounded to the storage type as well, being an operand of
+both products (the bias gradient sums it unrounded): in bf16 dx and dw of 32400 x 512 -> 2048 are 2.3e-3 off, of
+which their own rounding is 1.7e-3.  Two operands for dz, high and low part, would double the products.
 
 Capturing a backward pass in a HIP graph follows torch's rule for any operator: no autograd graph
 over the same leaves may be alive outside the capture.
