@@ -13,7 +13,9 @@ struct Plan {
 };
 
 // Time (us, without the launch) of t workgroups of a tile's kernel, each `per` steps of 128 bytes of k,
-// on the busiest CU; fitted to 40 sizes from 64 x 64 x 64 to 8192^3.  Two 16-bit 128 x 128 tiles share a
+// on the busiest CU; fitted to timings of each tile at 41 sizes from 64 x 64 x 64 to 8192^3, where the tile of
+// least cost comes within 10 % (or half a us) of the fastest, but for two sizes of 64 and 128 columns (13 %):
+// profiles/token_ops_tile_costs.csv.  Two 16-bit 128 x 128 tiles share a
 // CU and take 1.3 times as long as one alone; a 256 x 256 tile reads its residual with nothing under it.
 double tile_cost(int tile, long long t, long long per, int dtype, bool residual) {
   const double n = (double)((t + 255) / 256), k = (double)per;
