@@ -54,8 +54,7 @@ def _check(x, weight, device):
     return n, k, code
 
 
-# Scratch bytes by sizes and by where in 16 bytes the operands start: plans depend on nothing else, and asking
-# anew costs a call twice what looking them up does.
+# Scratch bytes by sizes and by where in 16 bytes the operands start, on which alone the plans depend: asked once.
 @functools.lru_cache(maxsize=4096)
 def _forward_scratch(x_at, ldx, weight_at, m, k, n, code, residual):
     return _lib.lib().sf_linear_workspace(x_at, ldx, weight_at, m, k, n, code, residual)
